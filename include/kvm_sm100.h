@@ -457,6 +457,33 @@ int kvm_sm100_kvcache_read(const void* cache, const kvm_kv_layout* layout, void*
                            void* v, const int32_t* kv_offsets, const int32_t* block_table,
                            const int32_t* bt_offsets, int S, int rows, kvm_stream_t stream);
 
+/* Page dst[i] of the pool := page src[i] for i < n, over `layers` layers from
+ * layout->layer on, K and V (device lists of page ids). A source may repeat.
+ * A pair whose page ids are out of range, whose destination another pair also
+ * writes, or whose destination another pair reads is skipped and reported
+ * through the device status, so the result does not depend on any order.
+ * token_stride must equal width. No counterpart in the reference: a caller
+ * that shares pages between sequences (the block tables are the caller's)
+ * gives a fork its own copy of the page it will write, or moves pages. */
+int kvm_sm100_kvcache_copy_pages(void* cache, const kvm_kv_layout* layout, int layers,
+                                 const int32_t* src, const int32_t* dst, int n,
+                                 kvm_stream_t stream);
+
+/* Keep some of the tokens written after position q_positions[s]: with kept =
+ * kept[kept_offsets[s]..kept_offsets[s+1]) (n_kept in all, strictly increasing
+ * from 0 in each sequence), the slot at position q_positions[s] + kept[i]
+ * moves to position q_positions[s] + i, over `layers` layers from
+ * layout->layer on, K and V: the accepted path of a drafted tree becomes the
+ * sequence's next tokens. In place. A sequence whose list is not strictly
+ * increasing, or with a position outside its table or a page outside the
+ * pool, is left as it is and reported through the device status. The pages
+ * moved to must not be shared between sequences of the call. No counterpart
+ * in the reference (it has no tree decoding). */
+int kvm_sm100_kvcache_compact(void* cache, const kvm_kv_layout* layout, int layers,
+                              const int32_t* kept, int n_kept, const int32_t* kept_offsets,
+                              const int32_t* q_positions, const int32_t* block_table,
+                              const int32_t* bt_offsets, int S, kvm_stream_t stream);
+
 /* kernel.attn.decode (dialect.cpp:39) over the paged cache, causal: query
  * row r of sequence s (rows q_offsets[s]..) at position p = q_positions[s]
  * + (r - q_offsets[s]) attends to cached positions 0..p of s (written
@@ -484,6 +511,62 @@ int kvm_sm100_attention_decode_paged(const void* q, int64_t ldq, const void* cac
  * base <= 0 selects 10000. */
 int kvm_sm100_rope_bf16(void* x, int64_t ld, int rows, int L, int heads,
                         int head_dim, float base, kvm_stream_t stream);
+
+/* Rotary position embedding with a position per row, the general form of
+ * kernel.attn.rope (dialect.cpp:40): for the pair i < rotary_dim/2 of a head,
+ *   theta = position * f_i,  (a, b) -> m (a cos - b sin, b cos + a sin);
+ * the pair is columns (2i, 2i+1) of the head (interleaved) or (i, i +
+ * rotary_dim/2); columns from rotary_dim on pass through. The frequencies
+ * start from f_i = base^(-2i/rotary_dim) and are stretched for contexts
+ * beyond the trained length by `scaling`:
+ *   KVM_ROPE_NONE      as they are
+ *   KVM_ROPE_LINEAR    f / factor
+ *   KVM_ROPE_NTK       base * factor^(d/(d-2)) in place of base
+ *   KVM_ROPE_BANDS     by the turns t = original_len * f / 2 pi a pair makes
+ *                      in the trained length: f / factor for t <= low, f for
+ *                      t >= high, linear in t between
+ *   KVM_ROPE_YARN      the same blend linear in i, from the pair that makes
+ *                      `high` turns (rounded down) to the one that makes `low`
+ *                      (rounded up); m = 0.1 ln(factor) + 1
+ *   KVM_ROPE_DIVISORS  f / divisors[i]
+ * magnitude > 0 replaces m (otherwise 1). */
+enum kvm_rope_scaling {
+  KVM_ROPE_NONE = 0, KVM_ROPE_LINEAR, KVM_ROPE_NTK, KVM_ROPE_BANDS, KVM_ROPE_YARN,
+  KVM_ROPE_DIVISORS
+};
+typedef struct kvm_rope_config {
+  int32_t rotary_dim; /* even, at most 2 * KVM_ROPE_MAX_PAIRS */
+  int32_t scaling;    /* kvm_rope_scaling */
+  double base, factor, original_len, low, high, magnitude;
+  const double* divisors; /* [rotary_dim / 2], host memory */
+} kvm_rope_config;
+
+/* The frequencies as 64-bit fractions of a turn (f / 2 pi * 2^64): position *
+ * turns[i] mod 2^64 is the angle, without the error a 32-bit product has at
+ * far positions. Host memory, copied into each launch: no device buffer. */
+#define KVM_ROPE_MAX_PAIRS 128
+typedef struct kvm_rope_table {
+  int32_t pairs;
+  float magnitude;
+  uint64_t turns[KVM_ROPE_MAX_PAIRS];
+} kvm_rope_table;
+
+/* Fill *table from *config (host only; once per model). */
+int kvm_sm100_rope_table(const kvm_rope_config* config, kvm_rope_table* table);
+
+/* out = rotated q, and with heads_k > 0 out_k = rotated k in the same launch.
+ * Rows hold heads of head_dim columns (even, at most 256), row strides in
+ * elements; dtype KVM_EW_BF16, F16 or F32 (the angle's cosine and sine and
+ * the products are fp32, rounded once). out may be the input itself with the
+ * same stride (rotation in place); other overlaps are undefined. positions:
+ * one per row, int32 or (positions_64) int64, of either sign. backward != 0
+ * applies the transposed rotation: the gradient of the forward call, and with
+ * m = 1 its inverse. */
+int kvm_sm100_rope(const kvm_rope_table* table, const void* q, int64_t ldq, void* out_q,
+                   int64_t ldoq, int heads_q, const void* k, int64_t ldk, void* out_k,
+                   int64_t ldok, int heads_k, int rows, int head_dim, int interleaved,
+                   int backward, int dtype, const void* positions, int positions_64,
+                   kvm_stream_t stream);
 
 /* ------------------------------------------------ graph execution helpers --- */
 

@@ -111,6 +111,11 @@ SIGNATURES = {
     "kvm_sm100_all_to_all": (_I, [_P, _P, _P, _I64, _I, _P]),
     "kvm_sm100_kvcache_write": (_I, [_P, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, _I, _I, _P]),
     "kvm_sm100_kvcache_read": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _P]),
+    "kvm_sm100_rope_table": (_I, [_P, _P]),
+    "kvm_sm100_rope": (_I, [_P, _P, _I64, _P, _I64, _I, _P, _I64, _P, _I64, _I, _I, _I, _I, _I,
+                            _I, _P, _I, _P]),
+    "kvm_sm100_kvcache_copy_pages": (_I, [_P, _P, _I, _P, _P, _I, _P]),
+    "kvm_sm100_kvcache_compact": (_I, [_P, _P, _I, _P, _I, _P, _P, _P, _P, _I, _P]),
     "kvm_sm100_attention_decode_workspace": (_I64, [_I, _I, _I, _I, _I]),
     "kvm_sm100_attention_decode_paged": (_I, [_P, _I64, _P, _P, _P, _I64, _P, _P, _P, _P,
                                               _I, _I, _I, _I, _F, _P, _I64, _P]),
@@ -134,6 +139,25 @@ class KvLayout(C.Structure):
                 ("kv_stride", C.c_int64), ("token_stride", C.c_int64),
                 ("block_size", C.c_int32), ("layer", C.c_int32), ("width", C.c_int32),
                 ("num_pages", C.c_int32)]
+
+
+KVM_ROPE_MAX_PAIRS = 128
+# enum kvm_rope_scaling (include/kvm_sm100.h)
+ROPE_SCALINGS = ["none", "linear", "ntk", "bands", "yarn", "divisors"]
+
+
+class RopeConfig(C.Structure):
+    """Mirror of struct kvm_rope_config (include/kvm_sm100.h)."""
+    _fields_ = [("rotary_dim", C.c_int32), ("scaling", C.c_int32), ("base", C.c_double),
+                ("factor", C.c_double), ("original_len", C.c_double), ("low", C.c_double),
+                ("high", C.c_double), ("magnitude", C.c_double),
+                ("divisors", C.POINTER(C.c_double))]
+
+
+class RopeTable(C.Structure):
+    """Mirror of struct kvm_rope_table (include/kvm_sm100.h)."""
+    _fields_ = [("pairs", C.c_int32), ("magnitude", C.c_float),
+                ("turns", C.c_uint64 * KVM_ROPE_MAX_PAIRS)]
 
 
 KVM_EW_MAX_INPUTS, KVM_EW_MAX_INSTR, KVM_EW_MAX_REGS = 8, 32, 16

@@ -30,6 +30,7 @@
 #include <cuda_bf16.h>
 
 #include "gemm_bf16.cuh"
+#include "kv_layout.h"
 #include "ptx.cuh"
 #include "runtime.h"
 
@@ -682,17 +683,6 @@ __global__ void kvcache_read_kernel(const __nv_bfloat16* __restrict__ cache,
   }
 }
 
-int check_layout(const kvm_kv_layout* L) {
-  if (!L) return fail(KVM_ERR_INVALID_ARG, "kv layout is NULL");
-  if (L->block_size < 1 || L->width <= 0 || L->width % 8 || L->num_pages <= 0 ||
-      L->layer < 0 || L->token_stride < L->width || L->token_stride % 8 ||
-      L->page_stride % 8 || L->layer_stride % 8 || L->kv_stride % 8)
-    return fail(KVM_ERR_INVALID_ARG,
-                "kv layout: need block_size >= 1, width % 8 == 0, 16-byte aligned "
-                "strides and token_stride >= width");
-  return KVM_OK;
-}
-
 }  // namespace
 }  // namespace kvm
 
@@ -703,7 +693,7 @@ extern "C" int kvm_sm100_kvcache_write(void* cache, const kvm_kv_layout* L, cons
                                        const int32_t* q_offsets, const int32_t* q_positions,
                                        const int32_t* block_table, const int32_t* bt_offsets,
                                        int S, int rows, kvm_stream_t stream) {
-  KVM_TRY(check_layout(L));
+  KVM_TRY(check_kv_layout(L));
   if (S <= 0 || rows < 0 || !cache || !k || !v || !q_offsets || !q_positions ||
       !block_table || !bt_offsets || !aligned16(cache) || !aligned16(k) || !aligned16(v) ||
       ldk < L->width || ldv < L->width || ldk % 8 || ldv % 8)
@@ -723,7 +713,7 @@ extern "C" int kvm_sm100_kvcache_read(const void* cache, const kvm_kv_layout* L,
                                       void* v, const int32_t* kv_offsets,
                                       const int32_t* block_table, const int32_t* bt_offsets,
                                       int S, int rows, kvm_stream_t stream) {
-  KVM_TRY(check_layout(L));
+  KVM_TRY(check_kv_layout(L));
   if (S <= 0 || rows < 0 || !cache || !k || !v || !kv_offsets || !block_table ||
       !bt_offsets || !aligned16(cache) || !aligned16(k) || !aligned16(v))
     return fail(KVM_ERR_INVALID_ARG, "kvcache_read: bad argument");
@@ -755,7 +745,7 @@ extern "C" int kvm_sm100_attention_decode_paged(
     const int32_t* block_table, const int32_t* bt_offsets, int S, int HQ, int max_q_rows,
     int max_keys, float scale, void* workspace, int64_t workspace_bytes,
     kvm_stream_t stream) {
-  KVM_TRY(check_layout(L));
+  KVM_TRY(check_kv_layout(L));
   if (S <= 0 || HQ <= 0 || L->width % 128 || HQ % (L->width / 128))
     return fail(KVM_ERR_INVALID_ARG,
                 "attention_decode: head_dim 128, width = HKV*128, HQ % HKV == 0");

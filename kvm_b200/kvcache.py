@@ -101,3 +101,46 @@ class PagedKVCache:
              bt_offsets.data_ptr(), S, heads_q, max_q_rows, max_keys, float(scale),
              workspace.data_ptr(), workspace.numel(), _stream())
         return out
+
+    def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """Page dst[i] := page src[i] in every layer, K and V (device int32
+        lists): a fork's own copy of the page it goes on writing, or pages
+        moved within the pool. Sources may repeat; a pair that would race with
+        another one (a destination named twice, or also a source) is skipped
+        and raises at the next ops.device_status(), as does a bad page id."""
+        for t, n in ((src, "src"), (dst, "dst")):
+            self._index(t, n)
+        if src.shape != dst.shape:
+            raise ValueError("src and dst must have the same length")
+        with torch.cuda.device(self.pool.device):
+            call("kvm_sm100_kvcache_copy_pages", self.pool.data_ptr(),
+                 C.byref(self.layout_struct(0)), self.layers, src.data_ptr(), dst.data_ptr(),
+                 src.numel(), _stream())
+
+    def compact(self, kept: torch.Tensor, kept_offsets: torch.Tensor,
+                q_positions: torch.Tensor, block_table: torch.Tensor,
+                bt_offsets: torch.Tensor) -> None:
+        """Keep the tokens kept[kept_offsets[s]:kept_offsets[s+1]] (strictly
+        increasing) of those written from position q_positions[s] on: token
+        kept[i] moves to position q_positions[s] + i in every layer. A sequence
+        with a bad list or page stays as it is and raises at the next
+        ops.device_status()."""
+        for t, n in ((kept, "kept"), (kept_offsets, "kept_offsets"),
+                     (q_positions, "q_positions"), (block_table, "block_table"),
+                     (bt_offsets, "bt_offsets")):
+            self._index(t, n)
+        S = q_positions.numel()
+        if kept_offsets.numel() != S + 1 or bt_offsets.numel() != S + 1:
+            raise ValueError("kept_offsets and bt_offsets must have one more entry than "
+                             "q_positions")
+        with torch.cuda.device(self.pool.device):
+            call("kvm_sm100_kvcache_compact", self.pool.data_ptr(),
+                 C.byref(self.layout_struct(0)), self.layers, kept.data_ptr(), kept.numel(),
+                 kept_offsets.data_ptr(), q_positions.data_ptr(), block_table.data_ptr(),
+                 bt_offsets.data_ptr(), S, _stream())
+
+    def _index(self, t: torch.Tensor, name: str) -> None:
+        """An int32 list on the pool's device."""
+        _check(t, name, torch.int32, 1)
+        if not t.is_contiguous() or t.device != self.pool.device:
+            raise ValueError(f"{name} must be contiguous on the pool's device")

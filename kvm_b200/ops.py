@@ -11,6 +11,7 @@ include/kvm_sm100.h.
 """
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass
 
 import torch
@@ -244,6 +245,91 @@ def rope_(x: torch.Tensor, *, seq_len: int, heads: int, head_dim: int = 128,
     return x
 
 
+_ROPE_DTYPE = {t: _lib.EW_DTYPES[n] for t, n in
+               ((torch.bfloat16, "bf16"), (torch.float16, "f16"), (torch.float32, "f32"))}
+
+
+def rope_table(rotary_dim: int, *, base: float = 10000.0, scaling: str = "none",
+               factor: float = 1.0, original_len: float = 0.0, low: float = 1.0,
+               high: float = 32.0, magnitude: float = 0.0, divisors=None) -> _lib.RopeTable:
+    """The rotary frequencies of a model for `rope` (made once, on the host).
+
+    scaling stretches them for contexts beyond the trained `original_len`:
+    "none", "linear", "ntk", "bands" (by a pair's turns in the trained length,
+    between `low` and `high`), "yarn" (the same blend by pair index, with its
+    magnitude 0.1 ln(factor) + 1) or "divisors" (one divisor per pair).
+    magnitude > 0 replaces the factor on the rotated values.
+    """
+    if scaling not in _lib.ROPE_SCALINGS:
+        raise ValueError(f"scaling must be one of {_lib.ROPE_SCALINGS}")
+    c = _lib.RopeConfig(int(rotary_dim), _lib.ROPE_SCALINGS.index(scaling), float(base),
+                        float(factor), float(original_len), float(low), float(high),
+                        float(magnitude))
+    if scaling == "divisors":
+        divisors = [float(d) for d in (divisors if divisors is not None else ())]
+        if len(divisors) != rotary_dim // 2:
+            raise ValueError("divisors must hold rotary_dim / 2 numbers")
+        c.divisors = (ctypes.c_double * len(divisors))(*divisors)
+    elif divisors is not None:
+        raise ValueError("divisors go with scaling='divisors'")
+    table = _lib.RopeTable()
+    call("kvm_sm100_rope_table", ctypes.byref(c), ctypes.byref(table))
+    return table
+
+
+def _rope_side(x, out, name, rows, heads, head_dim, like):
+    """Checks one of rope's tensors; returns its output."""
+    _check(x, name, like.dtype, 2)
+    if x.shape[0] != rows or x.shape[1] != heads * head_dim or x.device != like.device:
+        raise ValueError(f"{name} must be [{rows}, {heads} * {head_dim}] on the device of q")
+    if out is None:
+        return torch.empty((rows, heads * head_dim), dtype=x.dtype, device=x.device)
+    _check(out, "out of " + name, x.dtype, 2)
+    if out.shape != x.shape or out.device != x.device:
+        raise ValueError(f"out of {name} must have its shape and device")
+    return out
+
+
+def rope(q: torch.Tensor, positions: torch.Tensor, table: _lib.RopeTable, *, heads: int,
+         head_dim: int = 128, interleaved: bool = False, backward: bool = False,
+         k: torch.Tensor | None = None, heads_kv: int = 0, out: torch.Tensor | None = None,
+         out_k: torch.Tensor | None = None):
+    """Rotary embedding of q [rows, heads*head_dim] at positions [rows] (int32
+    or int64), and of k [rows, heads_kv*head_dim] in the same launch.
+
+    bf16, fp16 or fp32; row views are ok; `out` may be the input (in place).
+    The first rotary_dim columns of each head turn (pairs (i, i + rotary_dim/2),
+    or (2i, 2i+1) if interleaved), the others are copied. backward=True applies
+    the transposed rotation (the gradient of q from the gradient of the result).
+    Returns the rotated q, or the pair (q, k).
+    """
+    if not isinstance(table, _lib.RopeTable):
+        raise TypeError("table must come from rope_table")
+    if not isinstance(q, torch.Tensor) or q.dtype not in _ROPE_DTYPE:
+        raise TypeError("q must be a bf16, fp16 or fp32 tensor")
+    if (k is None) != (heads_kv == 0):
+        raise ValueError("k and heads_kv go together")
+    if q.dim() != 2:
+        raise ValueError(f"q must be 2-D, got shape {tuple(q.shape)}")
+    rows = q.shape[0]
+    out = _rope_side(q, out, "q", rows, heads, head_dim, q)
+    if k is not None:
+        out_k = _rope_side(k, out_k, "k", rows, heads_kv, head_dim, q)
+    if not positions.is_cuda or positions.dtype not in (torch.int32, torch.int64) or \
+            positions.shape != (rows,) or not positions.is_contiguous() or \
+            positions.device != q.device:
+        raise ValueError("positions must be contiguous int32 or int64 [rows] on q's device")
+    with torch.cuda.device(q.device):
+        call("kvm_sm100_rope", ctypes.byref(table), q.data_ptr(), _rowmajor(q, "q"),
+             out.data_ptr(), _rowmajor(out, "out"), heads,
+             _ptr(k), 0 if k is None else _rowmajor(k, "k"),
+             _ptr(out_k) if k is not None else None,
+             0 if k is None else _rowmajor(out_k, "out_k"), heads_kv, rows, head_dim,
+             int(interleaved), int(backward), _ROPE_DTYPE[q.dtype], positions.data_ptr(),
+             int(positions.dtype == torch.int64), _stream())
+    return out if k is None else (out, out_k)
+
+
 # ------------------------------------------------------------ elementwise ---
 
 def rmsnorm(x: torch.Tensor, gamma: torch.Tensor | None = None, eps: float = 1e-5,
@@ -414,7 +500,6 @@ def elementwise(instrs, inputs, out_shape, out_dtype: torch.dtype = torch.bfloat
     ins = _lib.EwInputs()
     for i, t in enumerate(inputs):
         ins.ptr[i] = t.data_ptr()
-    import ctypes
     call("kvm_sm100_elementwise", ctypes.byref(prog), ctypes.byref(ins), out.data_ptr(),
          out.numel(), _stream())
     return out
@@ -427,7 +512,7 @@ def device_status() -> int:
 
 __all__ = [
     "matmul", "gemm", "pack_gate_up", "quantize_e4m3", "matmul_fp8", "transpose_u8",
-    "transpose_f32", "attention_prefill", "rope_", "transpose", "silu_gate_matmul", "rmsnorm",
+    "transpose_f32", "attention_prefill", "rope_", "rope_table", "rope", "transpose", "silu_gate_matmul", "rmsnorm",
     "silu_mul", "moe_route", "moe_permute", "moe_scatter_rows", "grouped_matmul",
     "moe_combine", "Routing", "Dispatch", "elementwise", "device_status", "KVM_B_KN", "KVM_B_NK",
 ]

@@ -1,0 +1,130 @@
+"""Host side of the serving operators: the rotary table against 50-digit
+arithmetic, and the refusals of the C ABI (no GPU)."""
+import ctypes as C
+from decimal import Decimal, getcontext
+
+import pytest
+
+from kvm_b200 import _lib, ops
+from kvm_b200._lib import KvmError
+
+PI = Decimal("3.14159265358979323846264338327950288419716939937510")
+
+
+def _turns(d, base=10000, factor=1, kind="none", orig=0, low=1, high=32, div=None):
+    """f_i / 2 pi in 50 digits."""
+    getcontext().prec = 50
+    D = Decimal
+    base = D(base)
+    if kind == "ntk":
+        base *= D(factor) ** (D(d) / D(d - 2))
+    fs = [base ** (D(-2 * i) / D(d)) for i in range(d // 2)]
+    if kind == "linear":
+        fs = [f / D(factor) for f in fs]
+    if kind == "bands":
+        keep = [min(max((D(orig) * f / (2 * PI) - D(low)) / (D(high) - D(low)), D(0)), D(1))
+                for f in fs]
+        fs = [f * k + f / D(factor) * (1 - k) for f, k in zip(fs, keep)]
+    if kind == "yarn":
+        lo, hi = (D(d) * (D(orig) / (2 * PI * D(b))).ln() / (2 * base.ln()) for b in (high, low))
+        lo = max(lo.to_integral_value("ROUND_FLOOR"), D(0))
+        hi = min(hi.to_integral_value("ROUND_CEILING"), D(d - 1))
+        keep = [1 - min(max((i - lo) / max(hi - lo, D("1e-3")), D(0)), D(1))
+                for i in range(d // 2)]
+        fs = [f * k + f / D(factor) * (1 - k) for f, k in zip(fs, keep)]
+    if kind == "divisors":
+        fs = [f / D(x) for f, x in zip(fs, div)]
+    return [f / (2 * PI) for f in fs]
+
+
+@pytest.mark.parametrize("d,kw,ref", [
+    (128, {}, {}),
+    (64, dict(base=500000.0), dict(base=500000)),
+    (256, dict(scaling="linear", factor=7.0), dict(kind="linear", factor=7)),
+    (80, dict(scaling="ntk", factor=4.0), dict(kind="ntk", factor=4)),
+    (128, dict(scaling="bands", factor=8.0, original_len=8192, low=1.0, high=4.0,
+               base=500000.0), dict(kind="bands", factor=8, orig=8192, low=1, high=4, base=500000)),
+    (64, dict(scaling="yarn", factor=32.0, original_len=4096),
+     dict(kind="yarn", factor=32, orig=4096)),
+    (8, dict(scaling="divisors", divisors=[1.0, 2.0, 3.5, 64.0]),
+     dict(kind="divisors", div=["1", "2", "3.5", "64"])),
+])
+def test_rope_table(d, kw, ref):
+    """Turns as 64-bit fractions: long double arithmetic has 64 bits, a dozen
+    roundings of a value below 2^62, so a few dozen units at most."""
+    t = ops.rope_table(d, **kw)
+    assert t.pairs == d // 2
+    for got, want in zip(t.turns, _turns(d, **ref)):
+        assert abs(int(want * 2 ** 64) - got) <= 64, (got, want)
+    if kw.get("scaling") == "yarn":
+        assert abs(t.magnitude - (0.1 * float(Decimal(32).ln()) + 1)) < 1e-6
+    else:
+        assert t.magnitude == 1.0
+    assert ops.rope_table(d, magnitude=1.25, **kw).magnitude == 1.25
+
+
+@pytest.mark.parametrize("d,kw", [
+    (0, {}), (7, {}), (258, {}), (64, dict(base=1.0)), (64, dict(base=float("nan"))),
+    (64, dict(scaling="linear", factor=0.5)), (64, dict(scaling="linear", factor=float("inf"))),
+    (64, dict(scaling="bands", factor=2.0)), (2, dict(scaling="ntk", factor=2.0)),
+    (64, dict(scaling="yarn", factor=2.0, original_len=100, low=4.0, high=4.0)),
+    (64, dict(magnitude=-1.0)), (4, dict(scaling="divisors", divisors=[1.0, 0.0])),
+])
+def test_rope_table_refuses(d, kw):
+    with pytest.raises(KvmError) as e:
+        ops.rope_table(d, **kw)
+    assert e.value.code == _lib.KVM_ERR_INVALID_ARG
+
+
+def test_rope_table_python_refusals():
+    with pytest.raises(ValueError):
+        ops.rope_table(64, scaling="other")
+    with pytest.raises(ValueError):
+        ops.rope_table(64, scaling="divisors", divisors=[1.0])
+    with pytest.raises(ValueError):
+        ops.rope_table(64, divisors=[1.0] * 32)
+
+
+def _rc(name, *args):
+    return getattr(_lib.lib(), "kvm_sm100_" + name)(*args)
+
+
+def test_rope_refuses_without_a_gpu():
+    t = C.byref(ops.rope_table(64))
+    P = 4096   # an aligned address that is never read
+    ok = [t, P, 128, P, 128, 2, None, 0, None, 0, 0, 4, 64, 0, 0, 0, P, 0, None]
+
+    def bad(**at):
+        args = list(ok)
+        for i, v in at.items():
+            args[int(i[1:])] = v
+        return _rc("rope", *args)
+    INV = _lib.KVM_ERR_INVALID_ARG
+    assert bad(a0=None) == INV and bad(a1=None) == INV and bad(a16=None) == INV
+    assert bad(a2=100) == INV            # row stride below heads * head_dim
+    assert bad(a5=0) == INV and bad(a12=62) == INV and bad(a12=65) == INV and bad(a12=258) == INV
+    assert bad(a15=3) == INV and bad(a1=P + 1) == INV and bad(a16=P + 2) == INV
+    assert bad(a4=192) == INV            # in place with two row strides
+    assert bad(a10=1) == INV             # key heads without a key tensor
+    assert bad(a11=-1) == INV and bad(a11=0) == _lib.KVM_OK
+
+
+def test_page_calls_refuse_without_a_gpu():
+    L = _lib.KvLayout(4096, 2048, 1024, 64, 16, 0, 64, 4)
+    P = 4096
+    INV = _lib.KVM_ERR_INVALID_ARG
+    copy = lambda *a: _rc("kvcache_copy_pages", *a)  # noqa: E731
+    assert copy(P, None, 1, P, P, 1, None) == INV
+    assert copy(None, C.byref(L), 1, P, P, 1, None) == INV
+    assert copy(P, C.byref(L), 0, P, P, 1, None) == INV
+    assert copy(P, C.byref(L), 1, P, P, -1, None) == INV
+    assert copy(P, C.byref(L), 1, None, P, 1, None) == INV
+    assert copy(P, C.byref(L), 1, None, None, 0, None) == _lib.KVM_OK
+    wide = _lib.KvLayout(8192, 4096, 2048, 128, 16, 0, 64, 4)
+    assert copy(P, C.byref(wide), 1, P, P, 1, None) in (_lib.KVM_ERR_UNSUPPORTED,
+                                                        _lib.KVM_ERR_CUDA)
+    comp = lambda *a: _rc("kvcache_compact", *a)  # noqa: E731
+    assert comp(P, C.byref(L), 1, None, 1, P, P, P, P, 1, None) == INV
+    assert comp(P, C.byref(L), 1, P, -1, P, P, P, P, 1, None) == INV
+    assert comp(P + 8, C.byref(L), 1, P, 1, P, P, P, P, 1, None) == INV
+    assert comp(P, C.byref(L), 1, None, 0, None, None, None, None, 1, None) == _lib.KVM_OK
