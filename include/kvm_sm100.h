@@ -376,6 +376,23 @@ int kvm_sm100_attention_prefill_bf16(const void* q, int64_t ldq, const void* k,
                                      void* workspace, int64_t workspace_bytes,
                                      kvm_stream_t stream);
 
+/* The same over packed sequences of different lengths: sequence s owns rows
+ * offsets[s]..offsets[s+1] of q, k, v and out (device memory, S+1 entries;
+ * lengths from 0 up, at most 1024 sequences), and row r attends to the rows
+ * of its sequence up to itself. head_dim 64 or 128, dtype KVM_EW_BF16 or
+ * KVM_EW_F16, at most 128 query heads per kv head; `rows` rows exist in the
+ * tensors, and rows that belong to no sequence are neither read into a result
+ * nor written. Softmax statistics and sums are fp32, P is rounded to dtype
+ * for the product with V. What a row does not see (later rows, other
+ * sequences) cannot reach it, NaN and infinities included. A sequence whose
+ * offsets are descending or outside [0, rows] is skipped and reported through
+ * the device status. No workspace. kernel.attn.prefill with the row offsets of
+ * an attn_meta value (src/ir/dialect/kernel/values.h:83-117). */
+int kvm_sm100_attention_packed(const void* q, int64_t ldq, const void* k, int64_t ldk,
+                               const void* v, int64_t ldv, void* out, int64_t ldo,
+                               const int32_t* offsets, int S, int rows, int HQ, int HKV,
+                               int head_dim, int dtype, float scale, kvm_stream_t stream);
+
 /* ------------------------------------------------------- collectives --- */
 
 /* The kernel dialect's collectives (src/ir/dialect/kernel/dialect.cpp:58-64,
@@ -503,6 +520,32 @@ int kvm_sm100_attention_decode_paged(const void* q, int64_t ldq, const void* cac
                                      int S, int HQ, int max_q_rows, int max_keys,
                                      float scale, void* workspace, int64_t workspace_bytes,
                                      kvm_stream_t stream);
+
+/* Attention of a tree of drafted tokens over the paged cache: rows
+ * q_offsets[s]..q_offsets[s+1] of q are the drafted tokens ("nodes") of
+ * sequence s, whose K and V were written at positions q_positions[s] + i
+ * (kvm_sm100_kvcache_write). Node i attends to all q_positions[s] tokens
+ * before the tree and to the nodes j with bit j % 32 of word j / 32 of its
+ * mask row set (mask: [rows, mask_words] device words; itself is not implied,
+ * bits from the node count on are ignored). A row that sees nothing gets
+ * zeros. One node with bit 0 set is plain decoding. Heads and layout as for
+ * kvm_sm100_attention_decode_paged, at most 128 query heads per kv head, 1024
+ * sequences and 1024 nodes. max_q_rows and max_keys (cached tokens and nodes)
+ * bound every sequence and size the workspace; a sequence beyond them, or
+ * with bad offsets, is skipped and reported through the device status; so are
+ * pages outside the pool, whose sequence's result is undefined. Slots past a
+ * sequence's last node and nodes a row does not see cannot reach it, NaN and
+ * infinities included. */
+int64_t kvm_sm100_attention_tree_workspace(int S, int HQ, int HKV, int max_q_rows,
+                                           int max_keys);
+int kvm_sm100_attention_tree_paged(const void* q, int64_t ldq, const void* cache,
+                                   const kvm_kv_layout* layout, void* out, int64_t ldo,
+                                   const int32_t* q_offsets, const int32_t* q_positions,
+                                   const uint32_t* mask, int mask_words,
+                                   const int32_t* block_table, const int32_t* bt_offsets,
+                                   int S, int rows, int HQ, int max_q_rows, int max_keys,
+                                   float scale, void* workspace, int64_t workspace_bytes,
+                                   kvm_stream_t stream);
 
 /* Rotary position embedding in place, rotate-half form: kernel.attn.rope
  * (dialect.cpp:40). Rows are tokens b*L + pos (row stride ld elements); heads

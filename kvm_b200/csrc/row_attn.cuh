@@ -1,0 +1,1052 @@
+// Attention of packed query rows on the tensor cores, for prompts of
+// different lengths (packed_attn.cu) and for drafted trees over the paged
+// cache (tree_attn.cu): O = softmax(scale Q K^T + mask) V per kv head, one
+// pass over the keys with the running maximum and sum of the softmax.
+//
+// Rows. All query heads that share a kv head are rows of the same tile: row
+// r of a tile is token r / group, head r % group (one 3-D TMA box), so a
+// short sequence or a small tree fills a tile and K/V are read once for the
+// whole group. A work item has up to two tiles of 128 rows ("streams").
+//
+//   warps 0-3, 4-7   softmax of stream 0 and 1, one thread per row: S row
+//                    from TMEM to registers, mask, running max m and sum l,
+//                    P = 2^(s - m) rounded to the input type over S's own
+//                    columns in TMEM; at the end O / l to global memory
+//   warp 8 (1 lane)  MMA issuer: S_x = Q_x K_j^T (shared memory operands),
+//                    O_x += P_x V_j (P from TMEM: shared memory carries Q, K
+//                    and V reads only, 96 bytes a clock at full MMA rate
+//                    instead of 160)
+//   warp 9           TMA producer of the K and V tiles (one ring for both)
+//   warp 10 (1 lane) TMA producer of the Q tiles
+//   warp 11          looks over each V tile that some row must not see whole
+//
+// Two streams keep the tensor cores fed: while one does its softmax, the
+// other's P V and next Q K^T run. In PAIR items the streams are two Q tiles
+// that read the same K/V tiles. An item with one Q tile runs as ALT: both
+// streams hold that tile and take the even and the odd key tiles, and stream
+// 0 merges the two results at the end. The issuer walks the streams through
+// the items independently, so the next item's first S is computed while the
+// other stream still finishes this one.
+//
+// P overwrites S in place, so S_x(j+1) is issued after P V_x(j): MMAs of one
+// thread execute in order. For the same reason S_x(j+1) being complete means
+// that P V_x(j) is, and O_x may then be rescaled without another barrier. O
+// is rescaled only when a row's max grew by more than 2^8 since its P values
+// were scaled (P <= 2^8 is exact in range for bf16 and fp16, and l is fp32).
+//
+// Masked keys: scores are replaced, not added to, so NaN or infinite keys
+// cannot reach a row that does not see them. Values are different, as 0 * NaN
+// = NaN in the product: warp 11 zeroes what is not finite in V tiles that
+// some row sees only in part (and rows past the sequence's end), and the
+// epilogue adds those elements to the rows that do see them.
+//
+// Every wait is bounded; a timeout sets the device status and the kernel
+// drains.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "ptx.cuh"
+#include "runtime.h"
+
+namespace kvm {
+
+constexpr int kRowThreads = 384;
+// Registers a thread after the warps have split up: 168 * 384 at launch.
+constexpr int kRowSoftmaxRegs = 216;    // warps 0-7
+constexpr int kRowControlRegs = 72;     // warps 8-11
+constexpr float kRowRescale = 8.0f;     // log2 units
+constexpr int kRowMaxSeqs = 1024;       // sequences of one call (tables in shared memory)
+constexpr int kRowMaxDirty = 10;        // V tiles of an item that a row sees in part
+constexpr int kRowBadBufs = 8;          // items whose bad-value lists can be alive
+constexpr int kRowMaxNodes = 1024;
+
+// Shared memory of one CTA for head width D.
+template <int D>
+struct RowSmem {
+  static constexpr int kHalves = D / 64;
+  static constexpr uint32_t kHalf = 128 * 64 * 2;            // 128 rows x 64 columns
+  static constexpr uint32_t kTile = kHalves * kHalf;
+  static constexpr int kStages = D == 128 ? 4 : 8;           // tiles of the K/V ring, K in the even ones
+  static constexpr uint32_t kOffQ = 0;                       // [2]
+  static constexpr uint32_t kOffKV = 2 * kTile;              // [kStages]
+  static constexpr uint32_t kOffTab = kOffKV + kStages * kTile;
+  static constexpr uint32_t kTabBytes = kRowMaxSeqs * 10 + 16;
+  static constexpr uint32_t kOffBad = kOffTab + kTabBytes;
+  static constexpr uint32_t kOffMl = kOffBad + kRowBadBufs * kRowMaxDirty * 16;
+  static constexpr uint32_t kOffPages = kOffMl + 2 * 128 * 8;
+  static constexpr uint32_t kPageSlots = 128;                // page ids read ahead
+  static constexpr uint32_t kOffBar = kOffPages + kPageSlots * 4;
+  // q_full[2] q_empty[2] kv_full[S] kv_empty[S] v_ok[S] s_full[2] p_full[2]
+  // o_full[2] o_free[2] alt_ml[2] looked[8] bad_free[8] drain
+  static constexpr int kBars = 3 * kStages + 14 + 2 * kRowBadBufs + 1;
+  static constexpr size_t bytes() { return 1024 + kOffBar + kBars * 8 + 16; }
+};
+
+struct RowParams {
+  int S, HQ, HKV, group;
+  int tile_tokens;       // tokens of a Q tile: 128 / group
+  int rows;              // rows of q and out
+  float scale_log2;
+  void* out;
+  long long ldo;
+  const int* q_off;      // [S+1]
+  int* status;
+  // values again, for the epilogue's rare path
+  const void* v;
+  long long ldv;
+  // ---- trees over the paged cache
+  const int* q_pos;      // [S] cached tokens before the tree
+  const unsigned* mask;  // [rows, words]
+  int words, max_nodes, max_keys;
+  const int* bt;
+  const int* bt_off;
+  int block_size, box_rows, num_pages, layer;
+  long long page_rows, layer_rows, kv_rows;  // strides in token slots
+  float* ws_o;           // [2 * grid][256][128]
+  float* ws_ml;          // [2 * grid][256][2]
+};
+
+// A stretch of work: tiles [t0, t0 + n) of the keys for up to two Q tiles.
+struct RowItem {
+  int s, kh;
+  int row0;              // row of q of stream 0's first token
+  int tok0;              // that token's index in its sequence (node index of a tree)
+  int ntok0, ntok1;      // tokens of the two Q tiles
+  int key0;              // prompts: row of the sequence's first key
+  int ctx, nodes;        // trees
+  int keys;              // keys of the sequence
+  int t0, n, n0, n1;
+  int alt;
+  int part;              // slot of a partial result, -1: the whole result
+
+  __device__ __forceinline__ int count(int x) const {
+    return alt ? (x ? n >> 1 : (n + 1) >> 1) : (x ? n1 : n0);
+  }
+  __device__ __forceinline__ int tile(int x, int i) const { return alt ? 2 * i + x : i; }
+  // Whether both streams use the item's key tile j.
+  __device__ __forceinline__ bool shared(int j) const { return !alt && j < n0 && j < n1; }
+};
+
+// Tables in shared memory, built once per CTA from the offsets on the device.
+struct RowTables {
+  int* start;            // prompts: first item of rank r's block; trees: first tile of s
+  int* count;            // prompts: items of the sequence of rank r
+  unsigned short* order; // prompts: sequence of rank r
+  int* total;            // items (prompts) or tiles (trees)
+};
+
+template <int D>
+__device__ __forceinline__ RowTables row_tables(uint8_t* smem) {
+  RowTables t;
+  uint8_t* p = smem + RowSmem<D>::kOffTab;
+  t.start = reinterpret_cast<int*>(p);
+  t.count = reinterpret_cast<int*>(p + kRowMaxSeqs * 4);
+  t.order = reinterpret_cast<unsigned short*>(p + kRowMaxSeqs * 8);
+  t.total = reinterpret_cast<int*>(p + kRowMaxSeqs * 10);
+  return t;
+}
+
+// ------------------------------------------------------------- prompts ---
+//
+// Items of a sequence of n items are its Q tile pairs; the i-th costs about i
+// key tiles. They are dealt heaviest first: by i from the longest sequence's
+// last down to 0, every sequence that has an i-th item in turn. With the
+// sequences ranked by n descending, r + 1 of them have the items of the
+// levels (n_{r+1}, n_r], which start at item sum_{i<r} (n_i - n_r).
+__device__ __forceinline__ void build_prompt_tables(const RowParams& p, RowTables t,
+                                                    int* scratch) {
+  const int per = 2 * p.tile_tokens;
+  for (int s = threadIdx.x; s < p.S; s += kRowThreads) {
+    const int a = p.q_off[s], b = p.q_off[s + 1];
+    const bool bad = a < 0 || b < a || b > p.rows;
+    if (bad && blockIdx.x == 0) atomicOr(p.status, kDevBadInput);
+    scratch[s] = bad ? 0 : static_cast<int>((static_cast<long long>(b - a) + per - 1) / per);
+  }
+  __syncthreads();
+  for (int s = threadIdx.x; s < p.S; s += kRowThreads) {
+    const int n = scratch[s];
+    int rank = 0;
+    for (int i = 0; i < p.S; ++i) {
+      const int m = scratch[i];
+      rank += m > n || (m == n && i < s);
+    }
+    t.order[rank] = static_cast<unsigned short>(s);
+    t.count[rank] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    int before = 0;  // items of the ranks before this chunk
+    for (int r0 = 0; r0 < p.S; r0 += 32) {
+      const int r = r0 + threadIdx.x;
+      const int n = r < p.S ? t.count[r] : 0;
+      int sum = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (static_cast<int>(threadIdx.x) >= o) sum += up;
+      }
+      if (r < p.S) t.start[r] = before + sum - n - r * n;
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (threadIdx.x == 0) *t.total = before;
+  }
+  __syncthreads();
+}
+
+struct PromptItems {
+  int round = 0;
+  // The CTA's next item: rounds of one item per CTA, every other one in
+  // reverse, so no CTA always gets a round's heaviest.
+  __device__ __forceinline__ bool next(const RowParams& p, const RowTables& t, RowItem& it) {
+    const int G = gridDim.x, b = blockIdx.x;
+    const int w = round * G + (round & 1 ? G - 1 - b : b);
+    ++round;
+    if (w >= *t.total * p.HKV) return false;
+    it.kh = w % p.HKV;
+    const int u = w / p.HKV;
+    int lo = 0, hi = p.S - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (t.start[mid] <= u) lo = mid; else hi = mid - 1;
+    }
+    const int i = u - t.start[lo];
+    const int q_item = t.count[lo] - 1 - i / (lo + 1);
+    it.s = t.order[i % (lo + 1)];
+    it.key0 = p.q_off[it.s];
+    it.keys = p.q_off[it.s + 1] - it.key0;
+    it.tok0 = q_item * 2 * p.tile_tokens;
+    it.row0 = it.key0 + it.tok0;
+    const int left = it.keys - it.tok0;
+    it.ntok0 = min(left, p.tile_tokens);
+    it.ntok1 = max(0, min(left - p.tile_tokens, p.tile_tokens));
+    it.ctx = it.nodes = 0;
+    it.t0 = 0;
+    it.n0 = (it.tok0 + it.ntok0 + 127) >> 7;
+    it.n1 = it.ntok1 > 0 ? (it.tok0 + it.ntok0 + it.ntok1 + 127) >> 7 : 0;
+    it.n = max(it.n0, it.n1);
+    it.alt = it.ntok1 == 0 && it.n > 1;
+    it.part = -1;
+    return true;
+  }
+};
+
+// --------------------------------------------------------------- trees ---
+//
+// The key tiles of all (sequence, query tile pair, kv head) in a row, in that
+// order, are cut into one stretch of equal length per CTA: every CTA streams
+// the same number of K/V tiles whatever the contexts. A stretch that begins
+// or ends inside an item leaves a partial result; the combine kernel joins
+// them.
+__device__ __forceinline__ int tree_pairs(const RowParams& p, int nodes) {
+  return (nodes + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+}
+
+// Key tiles of sequence s, 0 for one that is empty or refused.
+__device__ __forceinline__ int tree_tiles(const RowParams& p, int s, int& nodes, int& ctx,
+                                          bool report) {
+  const int a = p.q_off[s], b = p.q_off[s + 1];
+  ctx = p.q_pos[s];
+  nodes = b - a;
+  const bool bad = a < 0 || b < a || b > p.rows || ctx < 0 || nodes > p.max_nodes ||
+                   ctx > p.max_keys - nodes;
+  if (bad && report) atomicOr(p.status, kDevBadInput);
+  if (bad || nodes == 0) { nodes = 0; return 0; }
+  return (ctx + nodes + 127) >> 7;
+}
+
+__device__ __forceinline__ void build_tree_tables(const RowParams& p, RowTables t, bool report) {
+  if (threadIdx.x < 32) {
+    int before = 0;
+    for (int s0 = 0; s0 < p.S; s0 += 32) {
+      const int s = s0 + threadIdx.x;
+      int n = 0;
+      if (s < p.S) {
+        int nodes, ctx;
+        const int tiles = tree_tiles(p, s, nodes, ctx, report);
+        n = tiles * tree_pairs(p, nodes) * p.HKV;
+      }
+      int sum = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (static_cast<int>(threadIdx.x) >= o) sum += up;
+      }
+      if (s < p.S) t.start[s] = before + sum - n;
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (threadIdx.x == 0) *t.total = before;
+  }
+  __syncthreads();
+}
+
+// Tiles per CTA: at least 4, so that small calls are not cut to pieces.
+__device__ __forceinline__ int tree_share(int total, int ctas) {
+  return max(4, (total + ctas - 1) / ctas);
+}
+
+struct TreeItems {
+  int pos = -1, end = 0, first = 1;
+  __device__ __forceinline__ bool next(const RowParams& p, const RowTables& t, RowItem& it) {
+    if (pos < 0) {
+      const int total = *t.total, share = tree_share(total, gridDim.x);
+      const long long b = static_cast<long long>(blockIdx.x) * share;
+      pos = b < total ? static_cast<int>(b) : total;
+      end = min(pos + share, total);
+    }
+    if (pos >= end) return false;
+    int lo = 0, hi = p.S - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (t.start[mid] <= pos) lo = mid; else hi = mid - 1;
+    }
+    it.s = lo;
+    const int tiles = tree_tiles(p, lo, it.nodes, it.ctx, false);
+    const int at = pos - t.start[lo];
+    const int item = at / tiles;
+    it.kh = item % p.HKV;
+    it.tok0 = item / p.HKV * 2 * p.tile_tokens;
+    it.key0 = 0;
+    it.row0 = p.q_off[lo] + it.tok0;
+    it.keys = it.ctx + it.nodes;
+    it.t0 = at - item * tiles;
+    it.n = min(tiles - it.t0, end - pos);
+    const int left = it.nodes - it.tok0;
+    it.ntok0 = min(left, p.tile_tokens);
+    it.ntok1 = max(0, min(left - p.tile_tokens, p.tile_tokens));
+    it.n0 = it.n;
+    it.n1 = it.ntok1 > 0 ? it.n : 0;
+    it.alt = it.ntok1 == 0 && it.n > 1;
+    it.part = it.n == tiles ? -1 : 2 * int(blockIdx.x) + (first ? 0 : 1);
+    first = 0;
+    pos += it.n;
+    return true;
+  }
+};
+
+// -------------------------------------------------------------- pieces ---
+
+// D[tmem] (+)= A[tmem] x B[smem desc]^T, kind::f16; A holds 128 rows of 16-bit
+// pairs, one row per lane.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                           uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 3-D tiled TMA load (x innermost).
+__device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, uint64_t* bar,
+                                            int32_t x, int32_t y, int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void reg_give() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_take() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+template <bool F16>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if constexpr (F16) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+template <bool F16>
+__host__ __device__ constexpr uint32_t row_idesc(int n, int b_mn) {
+  const uint32_t type = F16 ? 0u : 1u;
+  return (1u << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(b_mn) << 16) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
+}
+
+// Bits of the mask of one tree row for the 32 keys from `rel` (the key's index
+// minus the cached ones) on: cached keys all seen, drafted ones by the mask.
+__device__ __forceinline__ unsigned tree_bits(const unsigned* mask, int words, int nodes,
+                                              int rel) {
+  if (rel <= -32) return 0xffffffffu;
+  if (rel >= nodes) return 0u;
+  const int w = rel >> 5;
+  const unsigned lo = w < 0 ? 0xffffffffu : w < words ? mask[w] : 0u;
+  const unsigned hi = w + 1 < words ? mask[w + 1] : 0u;
+  unsigned bits = __funnelshift_r(lo, hi, rel & 31);
+  const int left = nodes - rel;  // keys of the sequence from rel on
+  if (left < 32) bits &= (1u << left) - 1u;
+  return bits;
+}
+
+// Whether row (token t of its sequence) sees key k.
+template <bool TREE>
+__device__ __forceinline__ bool row_sees(const RowItem& it, const unsigned* mask, int words,
+                                         int token, int k) {
+  if constexpr (!TREE) return k <= token;
+  if (k < it.ctx) return true;
+  const int j = k - it.ctx;
+  return j < it.nodes && (j >> 5) < words && (mask[j >> 5] >> (j & 31) & 1u);
+}
+
+// First key tile (relative to the item's) that some row sees only in part.
+template <bool TREE>
+__device__ __forceinline__ int first_dirty(const RowItem& it) {
+  const int k = TREE ? it.ctx : it.tok0 + 1;  // first key not seen by all
+  return max(0, (k >> 7) - it.t0);
+}
+
+// Address of the value row of key k (the epilogue's rare path), or NULL.
+template <bool TREE>
+__device__ __forceinline__ const uint16_t* value_row(const RowParams& p, const RowItem& it,
+                                                     int D, int k) {
+  long long row = it.key0 + k;
+  if constexpr (TREE) {
+    const int idx = k / p.block_size, b0 = p.bt_off[it.s];
+    const int page = idx < p.bt_off[it.s + 1] - b0 ? p.bt[b0 + idx] : -1;
+    if (page < 0 || page >= p.num_pages) return nullptr;
+    row = page * p.page_rows + p.layer * p.layer_rows + p.kv_rows + k % p.block_size;
+  }
+  return static_cast<const uint16_t*>(p.v) + row * p.ldv + static_cast<long long>(it.kh) * D;
+}
+
+template <bool F16>
+__device__ __forceinline__ bool nonfinite16(uint16_t b) {
+  constexpr uint16_t top = F16 ? 0x7C00 : 0x7F80;
+  return (b & top) == top;
+}
+template <bool F16>
+__device__ __forceinline__ float widen16(uint16_t b) {
+  if constexpr (F16) return __half2float(*reinterpret_cast<const __half*>(&b));
+  else return __uint_as_float(static_cast<uint32_t>(b) << 16);
+}
+
+// -------------------------------------------------------------- kernel ---
+
+template <int D, bool F16, bool TREE>
+__global__ void __launch_bounds__(kRowThreads, 1)
+    row_attn_kernel(const __grid_constant__ CUtensorMap tmQ,
+                    const __grid_constant__ CUtensorMap tmK,
+                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ RowParams p) {
+  using L = RowSmem<D>;
+  using Items = typename std::conditional<TREE, TreeItems, PromptItems>::type;
+  constexpr int NST = L::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+  uint64_t* q_full = bars;                      // [2]
+  uint64_t* q_empty = q_full + 2;               // [2]
+  uint64_t* kv_full = q_empty + 2;              // [NST]
+  uint64_t* kv_empty = kv_full + NST;           // [NST]
+  uint64_t* v_ok = kv_empty + NST;              // [NST] 32 arrivals
+  uint64_t* s_full = v_ok + NST;                // [2]
+  uint64_t* p_full = s_full + 2;                // [2] 128 arrivals
+  uint64_t* o_full = p_full + 2;                // [2]
+  uint64_t* o_free = o_full + 2;                // [2] 128 arrivals
+  uint64_t* alt_ml = o_free + 2;                // [2] 128 arrivals
+  uint64_t* looked = alt_ml + 2;                // [kRowBadBufs] 32 arrivals
+  uint64_t* bad_free = looked + kRowBadBufs;    // [kRowBadBufs] 8 arrivals
+  uint64_t* drain = bad_free + kRowBadBufs;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  unsigned* bad_words = reinterpret_cast<unsigned*>(smem + L::kOffBad);
+  float2* alt_buf = reinterpret_cast<float2*>(smem + L::kOffMl);   // [2][128]
+  const RowTables tab = row_tables<D>(smem);
+
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 2 - i);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&o_free[i], 128);
+      mbar_init(&alt_ml[i], 128);
+    }
+    for (int i = 0; i < NST; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 2);
+      mbar_init(&v_ok[i], 32);
+    }
+    for (int i = 0; i < kRowBadBufs; ++i) {
+      mbar_init(&looked[i], 32);
+      mbar_init(&bad_free[i], 8);
+    }
+    mbar_init(drain, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if constexpr (TREE) build_tree_tables(p, tab, blockIdx.x == 0);
+  else build_prompt_tables(p, tab, reinterpret_cast<int*>(smem + L::kOffKV));
+  fence_async_smem();  // the tables' scratch becomes a tile of the ring
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // columns: S_0 (P_0 over its first half), S_1, O_0, O_1
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 8) {
+    reg_give<kRowControlRegs>();
+    if (warp == 9) {
+      // ------------------------------------------------ K/V producer
+      int* page_ids = reinterpret_cast<int*>(smem + L::kOffPages);
+      Items items;
+      RowItem it;
+      uint32_t c = 0;  // ring slots filled
+      bool ok = true;
+      while (ok && items.next(p, tab, it)) {
+        int have = -1;  // page ids [have, have + kPageSlots) of the sequence are in shared memory
+        for (int j = 0; j < it.n && ok; ++j) {
+          const int k0 = (it.t0 + j) * 128;
+          if constexpr (TREE) {
+            const int k1 = min(k0 + 128, it.keys);
+            const int pg0 = k0 / p.block_size, pg1 = (k1 - 1) / p.block_size;
+            if (have < 0 || pg1 >= have + static_cast<int>(L::kPageSlots)) {
+              have = pg0;
+              const int bt0 = p.bt_off[it.s], bt_n = p.bt_off[it.s + 1] - bt0;
+              const int last = min(have + static_cast<int>(L::kPageSlots),
+                                   (it.keys - 1) / p.block_size + 1);
+              __syncwarp();
+              for (int i = have + lane; i < last; i += 32) {
+                const int page = i < bt_n ? p.bt[bt0 + i] : -1;
+                // Pages outside the pool or the table are reported and not
+                // loaded: every access stays inside the pool, and what the
+                // sequence's rows get is undefined.
+                const bool good = page >= 0 && page < p.num_pages;
+                if (!good) atomicOr(p.status, kDevBadInput);
+                page_ids[i - have] = good ? page : -1;
+              }
+              __syncwarp();
+            }
+            const int segs = (k1 - k0 + p.box_rows - 1) / p.box_rows;
+            const int tok = k0 + lane * p.box_rows;
+            const int page = lane < segs ? page_ids[tok / p.block_size - have] : -1;
+            const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
+            const uint32_t bytes = boxes * p.box_rows * (D * 2u);
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+              const uint32_t st = c % NST;
+              bool got = true;
+              if (lane == 0) {
+                got = mbar_wait(&kv_empty[st], ((c / NST) & 1) ^ 1, abort_flag);
+                if (got) mbar_arrive_expect_tx(&kv_full[st], bytes);
+              }
+              ok = __shfl_sync(0xffffffffu, got, 0);
+              if (!ok) break;
+              if (page >= 0) {
+                const int row = static_cast<int>(page * p.page_rows + p.layer * p.layer_rows +
+                                                 kv * p.kv_rows + tok % p.block_size);
+                uint8_t* dst = smem + L::kOffKV + st * L::kTile + lane * p.box_rows * 128u;
+#pragma unroll
+                for (int h = 0; h < L::kHalves; ++h)
+                  tma_load_2d(dst + h * L::kHalf, &tmK, &kv_full[st], it.kh * D + h * 64, row);
+              }
+              ++c;
+            }
+          } else if (lane == 0) {
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+              const uint32_t st = c % NST;
+              if (!mbar_wait(&kv_empty[st], ((c / NST) & 1) ^ 1, abort_flag)) {
+                ok = false;
+                break;
+              }
+              mbar_arrive_expect_tx(&kv_full[st], L::kTile);
+              uint8_t* dst = smem + L::kOffKV + st * L::kTile;
+#pragma unroll
+              for (int h = 0; h < L::kHalves; ++h)
+                tma_load_2d(dst + h * L::kHalf, kv ? &tmV : &tmK, &kv_full[st],
+                            it.kh * D + h * 64, it.key0 + k0);
+              ++c;
+            }
+          }
+        }
+        __syncwarp();
+      }
+    } else if (warp == 10) {
+      if (lane == 0) {
+        // ---------------------------------------------- Q producer
+        Items items;
+        RowItem it;
+        uint32_t uses0 = 0, uses1 = 0;
+        const uint32_t bytes = L::kHalves * 64u * 2u * p.group * p.tile_tokens;
+        bool ok = true;
+        while (ok && items.next(p, tab, it)) {
+          for (int x = 0; x < 2 && ok; ++x) {
+            if (x == 1 && it.n1 == 0) break;
+            uint32_t& uses = x ? uses1 : uses0;
+            if (!mbar_wait(&q_empty[x], (uses & 1) ^ 1, abort_flag)) { ok = false; break; }
+            ++uses;
+            mbar_arrive_expect_tx(&q_full[x], bytes);
+            for (int h = 0; h < L::kHalves; ++h)
+              tma_load_3d(smem + L::kOffQ + x * L::kTile + h * L::kHalf, &tmQ, &q_full[x],
+                          h * 64, it.kh * p.group, it.row0 + x * p.tile_tokens);
+          }
+        }
+      }
+    } else if (warp == 11) {
+      // ------------------------------------------------ value tiles
+      Items items;
+      RowItem it;
+      uint32_t c = 0, ord = 0;
+      bool ok = true;
+      while (ok && items.next(p, tab, it)) {
+        const int dirty = first_dirty<TREE>(it);
+        unsigned* bad = bad_words + (ord % kRowBadBufs) * (kRowMaxDirty * 4);
+        const bool free = mbar_wait(&bad_free[ord % kRowBadBufs],
+                                    ((ord / kRowBadBufs) & 1) ^ 1, abort_flag);
+        if (!__all_sync(0xffffffffu, free)) break;
+        for (int j = 0; j < it.n; ++j, ++c) {
+          const uint32_t slot = 2 * c + 1, st = slot % NST;
+          const bool in = mbar_wait(&kv_full[st], (slot / NST) & 1, abort_flag);
+          if (!__all_sync(0xffffffffu, in)) { ok = false; break; }
+          if (j >= dirty) {
+            uint8_t* tile = smem + L::kOffKV + st * L::kTile;
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q) {
+              const int r = q * 32 + lane;
+              const int key = (it.t0 + j) * 128 + r;
+              bool found = false;
+#pragma unroll
+              for (int h = 0; h < L::kHalves; ++h) {
+                uint8_t* row = tile + h * L::kHalf + r * 128;
+                if (key >= it.keys) {
+#pragma unroll
+                  for (int ch = 0; ch < 8; ++ch)
+                    *reinterpret_cast<uint4*>(row + ((ch ^ (r & 7)) << 4)) =
+                        make_uint4(0, 0, 0, 0);
+                } else {
+                  // the largest magnitude of the half row, two values at a time
+                  unsigned top = 0;
+#pragma unroll
+                  for (int ch = 0; ch < 8; ++ch) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(row + ((ch ^ (r & 7)) << 4));
+                    top = __vmaxu2(top, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu),
+                                                 __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
+                  }
+                  constexpr unsigned inf = F16 ? 0x7C00u : 0x7F80u;
+                  if ((top & 0xFFFFu) >= inf || (top >> 16) >= inf) {
+                    found = true;
+                    uint16_t* e = reinterpret_cast<uint16_t*>(row);
+                    for (int i = 0; i < 64; ++i)
+                      if (nonfinite16<F16>(e[i])) e[i] = 0;
+                  }
+                }
+              }
+              const unsigned word = __ballot_sync(0xffffffffu, found);
+              if (lane == 0 && j - dirty < kRowMaxDirty) bad[(j - dirty) * 4 + q] = word;
+            }
+            fence_async_smem();
+          }
+          mbar_arrive(&v_ok[st]);
+        }
+        if (!ok) break;
+        mbar_arrive(&looked[ord % kRowBadBufs]);
+        ++ord;
+      }
+    } else if (lane == 0) {
+      // ------------------------------------------------ MMA issuer
+      constexpr uint32_t kIdescQK = row_idesc<F16>(128, 0);
+      constexpr uint32_t kIdescPV = row_idesc<F16>(D, 1);
+      // Each stream has a cursor: the key tile it is at, and whether S or P V
+      // comes next there.
+      struct Cursor {
+        Items items;
+        RowItem it;
+        bool live, scored;   // scored: S of the tile is issued, P V comes next
+        int i, cnt;          // position in the stream's tiles of the item
+        uint32_t base;       // key tiles of the items before
+        uint32_t ord0, ord1; // items so far that used Q tile 0 (all) / 1
+        uint32_t tiles;      // tiles of the stream so far
+        uint32_t mine;       // items of the stream so far
+      };
+      Cursor cur[2];
+      bool ok = true;
+      // The stream's next item with work for it.
+      auto advance = [&](Cursor& c, int x, bool begin) {
+        for (;;) {
+          if (!begin) {
+            c.base += c.it.n;
+            ++c.ord0;
+            c.ord1 += c.it.n1 > 0;
+          }
+          begin = false;
+          c.live = c.items.next(p, tab, c.it);
+          if (!c.live) return;
+          c.i = 0;
+          c.scored = false;
+          c.cnt = c.it.count(x);
+          if (c.cnt > 0) return;
+        }
+      };
+      // Whether the stream's next step may be waited for with the other stream
+      // where it is. The ring holds kStages / 2 >= 2 key tiles and is filled in
+      // order: K of tile g needs every S up to g - 2 and every P V up to g - 3
+      // issued, V of tile g every P V up to g - 2. An item's Q tiles are loaded
+      // once every S of the items before is issued. The first P V of an item
+      // waits for the epilogue of the one before, which in an ALT item needs
+      // both streams' P V. The stream that is behind may always go on.
+      auto may = [&](const Cursor& c, int x, const Cursor& o, int ox) {
+        if (!o.live) return true;
+        const int g = c.base + c.it.tile(x, c.i), og = o.base + o.it.tile(ox, o.i);
+        if (!c.scored)
+          return og >= g - (o.scored ? 2 : 1) &&
+                 (c.i > 0 || o.ord0 >= c.ord0 ||
+                  (o.ord0 + 1 == c.ord0 && o.scored && o.i == o.cnt - 1));
+        return og >= g - 1 && (c.i > 0 || o.ord0 >= c.ord0);
+      };
+      auto issue_s = [&](Cursor& c, int x) {
+        const int j = c.it.tile(x, c.i);
+        const int qt = c.it.alt ? 0 : x;
+        const uint32_t slot = 2 * (c.base + j), st = slot % NST;
+        if ((c.i == 0 && !mbar_wait(&q_full[qt], (qt ? c.ord1 : c.ord0) & 1, abort_flag)) ||
+            !mbar_wait(&kv_full[st], (slot / NST) & 1, abort_flag)) {
+          ok = false;
+          return;
+        }
+        tc_fence_after();
+        const uint32_t q_addr = smem_u32(smem + L::kOffQ + qt * L::kTile);
+        const uint32_t k_addr = smem_u32(smem + L::kOffKV + st * L::kTile);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * L::kHalf + (kk & 3) * 32;
+          mma_f16_ss(tmem + x * 128, sdesc_sw128(q_addr + off, 0, 1024),
+                     sdesc_sw128(k_addr + off, 0, 1024), kIdescQK, kk > 0);
+        }
+        mma_commit(&s_full[x]);
+        // Two arrivals free a slot: one of each stream, or both of its only one.
+        mma_commit(&kv_empty[st]);
+        if (!c.it.shared(j)) mma_commit(&kv_empty[st]);
+        if (c.i == c.cnt - 1) {
+          mma_commit(&q_empty[qt]);
+          if (qt == 0 && !c.it.alt) mma_commit(&q_empty[0]);
+        }
+        c.scored = true;
+      };
+      auto issue_pv = [&](Cursor& c, int x) {
+        const int j = c.it.tile(x, c.i);
+        const uint32_t slot = 2 * (c.base + j) + 1, st = slot % NST;
+        if (!mbar_wait(&p_full[x], c.tiles & 1, abort_flag) ||
+            (c.i == 0 && !mbar_wait(&o_free[x], (c.mine & 1) ^ 1, abort_flag)) ||
+            !mbar_wait(&kv_full[st], (slot / NST) & 1, abort_flag) ||
+            !mbar_wait(&v_ok[st], (slot / NST) & 1, abort_flag)) {
+          ok = false;
+          return;
+        }
+        tc_fence_after();
+        const uint32_t v_addr = smem_u32(smem + L::kOffKV + st * L::kTile);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          mma_f16_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8,
+                     sdesc_sw128(v_addr + kk * 2048, L::kHalf, 1024), kIdescPV,
+                     (c.i > 0 || kk > 0) ? 1u : 0u);
+        mma_commit(&kv_empty[st]);
+        if (!c.it.shared(j)) mma_commit(&kv_empty[st]);
+        if (c.i == c.cnt - 1) mma_commit(&o_full[x]);
+        ++c.tiles;
+        c.scored = false;
+        if (++c.i == c.cnt) {
+          ++c.mine;
+          advance(c, x, false);
+        }
+      };
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        cur[x].base = cur[x].ord0 = cur[x].ord1 = cur[x].tiles = cur[x].mine = 0;
+        advance(cur[x], x, true);
+      }
+      while (ok && (cur[0].live || cur[1].live)) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          Cursor& c = cur[x];
+          const Cursor& o = cur[1 - x];
+          if (ok && c.live && c.scored && may(c, x, o, 1 - x)) issue_pv(c, x);
+          if (ok && c.live && !c.scored && may(c, x, o, 1 - x)) issue_s(c, x);
+        }
+      }
+      // Every MMA issued above must finish before TMEM is released.
+      mma_commit(drain);
+      volatile int local_abort = 0;
+      mbar_wait(drain, 0, &local_abort);
+    }
+  } else {
+    // ------------------------------------------------ softmax / epilogue
+    reg_take<kRowSoftmaxRegs>();
+    const int x = warp >> 2;
+    const int quarter = warp & 3;               // TMEM lane quarter
+    const int r = quarter * 32 + lane;          // row of the Q tile
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t tS = tmem + x * 128 + lanes, tP = tS, tO = tmem + 256 + x * 128 + lanes;
+    const float sl2 = p.scale_log2;
+    const int r_tok = r / p.group, r_head = r - r_tok * p.group;
+    Items items;
+    RowItem it;
+    uint32_t tiles = 0, mine = 0, act1 = 0, alts = 0, ord = 0;
+    bool ok = true;
+    for (; ok && items.next(p, tab, it); ++ord) {
+      const int cnt = it.count(x);
+      if (cnt == 0) {
+        // Looked at, so the list of eight items ago has been given back by both
+        // streams: this arrival cannot be taken for that item's.
+        const bool seen = mbar_wait(&looked[ord % kRowBadBufs], (ord / kRowBadBufs) & 1, abort_flag);
+        if (!__all_sync(0xffffffffu, seen)) break;
+        if (lane == 0) mbar_arrive(&bad_free[ord % kRowBadBufs]);
+        continue;
+      }
+      const int q_tile = it.alt ? 0 : x;
+      const int token = it.tok0 + q_tile * p.tile_tokens + r_tok;   // in its sequence
+      const unsigned* mask = nullptr;
+      if constexpr (TREE)  // rows past the tree's end read the last node's mask
+        mask = p.mask + static_cast<long long>(p.q_off[it.s] + min(token, it.nodes - 1)) * p.words;
+      float m = -INFINITY, msl = 0.f;
+      float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      for (int i = 0; i < cnt; ++i) {
+        const bool ready = mbar_wait(&s_full[x], tiles & 1, abort_flag);
+        ++tiles;
+        if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
+        tc_fence_after();
+        float s[128];
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4)
+          tmem_ld32(tS + c4 * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c4 * 32]));
+        tmem_wait_ld();
+        const int k0 = (it.t0 + it.tile(x, i)) * 128;
+        if constexpr (TREE) {
+          if (k0 + 128 > it.ctx) {
+#pragma unroll
+            for (int c4 = 0; c4 < 4; ++c4) {
+              const unsigned bits = tree_bits(mask, p.words, it.nodes, k0 + c4 * 32 - it.ctx);
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                if (!(bits >> c & 1u)) s[c4 * 32 + c] = -INFINITY;
+            }
+          }
+        } else {
+          if (k0 + 127 > it.tok0 + q_tile * p.tile_tokens) {
+            const int lim = token - k0;
+#pragma unroll
+            for (int c = 0; c < 128; ++c)
+              if (c > lim) s[c] = -INFINITY;
+          }
+        }
+        // Row max as four chains (max is exact in any order).
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int c = 4; c < 128; c += 4)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], s[c + u]);
+        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if (i == 0) {
+          m = mt;
+          msl = m == -INFINITY ? 0.f : m * sl2;
+        } else if (__any_sync(0xffffffffu, (mt - m) * sl2 > kRowRescale ||
+                                               (m == -INFINITY && mt > -INFINITY))) {
+          const float mn = fmaxf(m, mt);
+          const float nsl = mn == -INFINITY ? 0.f : mn * sl2;
+          const float alpha = m == -INFINITY ? 0.f : ex2_approx(msl - nsl);
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            uint32_t u[16];
+            tmem_ld16(tO + c, u);
+            tmem_wait_ld();
+#pragma unroll
+            for (int q = 0; q < 16; ++q)
+              u[q] = __float_as_uint(__uint_as_float(u[q]) * alpha);
+            tmem_st16(tO + c, u);
+          }
+          l2[0].x *= alpha; l2[0].y *= alpha; l2[1].x *= alpha; l2[1].y *= alpha;
+          m = mn;
+          msl = nsl;
+        }
+        // P = 2^(s scale - m), two at a time, rounded to the input type for the
+        // product with V; l sums the unrounded values.
+        const float2 sc = make_float2(sl2, sl2), neg = make_float2(-msl, -msl);
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4) {
+          uint32_t u[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            float2 e = __ffma2_rn(make_float2(s[c4 * 32 + 2 * c], s[c4 * 32 + 2 * c + 1]), sc, neg);
+            e.x = ex2_approx(e.x);
+            e.y = ex2_approx(e.y);
+            l2[c & 1] = __fadd2_rn(l2[c & 1], e);
+            u[c] = pack16<F16>(e.x, e.y);
+          }
+          tmem_st16(tP + c4 * 16, u);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[x]);
+      }
+      if (!ok) break;
+      float l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+      if (it.alt && x == 1) {
+        alt_buf[(alts & 1) * 128 + r] = make_float2(m == -INFINITY ? m : msl, l);
+        mbar_arrive(&alt_ml[alts & 1]);
+        const bool seen = mbar_wait(&looked[ord % kRowBadBufs], (ord / kRowBadBufs) & 1, abort_flag);
+        if (!__all_sync(0xffffffffu, seen)) break;
+        if (lane == 0) mbar_arrive(&bad_free[ord % kRowBadBufs]);
+        ++alts;
+        ++mine;
+        continue;
+      }
+      // ---- epilogue
+      bool fin = mbar_wait(&o_full[x], mine & 1, abort_flag);
+      float a0 = 1.f, a1 = 0.f;                  // weights of the two streams' O
+      float ml = m == -INFINITY ? m : msl;       // running max, log2 units
+      if (it.alt) {
+        fin = fin && mbar_wait(&o_full[1], act1 & 1, abort_flag) &&
+              mbar_wait(&alt_ml[alts & 1], (alts >> 1) & 1, abort_flag);
+        if (__all_sync(0xffffffffu, fin)) {
+          const float2 o = alt_buf[(alts & 1) * 128 + r];
+          const float mm = fmaxf(ml, o.x);
+          // a stream that saw nothing has m = -inf and O = 0
+          a0 = ml == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : ex2_approx(ml - mm);
+          a1 = o.x == -INFINITY ? 0.f : ex2_approx(o.x - mm);
+          l = l * a0 + o.y * a1;
+          ml = mm;
+        }
+        ++alts;
+      }
+      fin = fin && mbar_wait(&looked[ord % kRowBadBufs], (ord / kRowBadBufs) & 1, abort_flag);
+      if (!__all_sync(0xffffffffu, fin)) { ok = false; break; }
+      ++mine;
+      act1 += it.count(1) > 0;
+      tc_fence_after();
+      const bool valid = r_tok < (q_tile ? it.ntok1 : it.ntok0) && r_tok < p.tile_tokens;
+      const int row = it.row0 + q_tile * p.tile_tokens + r_tok;
+      const int head = it.kh * p.group + r_head;
+      // Values that are not finite, of keys this row sees (words of the item's
+      // dirty tiles; all zero but for broken inputs).
+      const unsigned* bad = bad_words + (ord % kRowBadBufs) * (kRowMaxDirty * 4);
+      const int dirty = first_dirty<TREE>(it);
+      const int bad_n = min(max(it.n - dirty, 0), kRowMaxDirty) * 4;
+      unsigned any_bad = 0;
+      for (int w = 0; w < bad_n; ++w) any_bad |= bad[w];
+      float inv = 1.0f;
+      if (it.part < 0) {
+        inv = 1.0f / l;
+        if constexpr (TREE) {
+          if (l == 0.f) {  // a row that sees no key at all is zero
+            bool sees = it.ctx > 0;
+            for (int w = 0; w < p.words && !sees; ++w)
+              sees = tree_bits(mask, p.words, it.nodes, w * 32) != 0;
+            if (!sees) inv = 0.f;
+          }
+        }
+      }
+#pragma unroll 1
+      for (int c4 = 0; c4 < D / 32; ++c4) {
+        uint32_t u[32];
+        tmem_ld32(tO + c4 * 32, u);
+        tmem_wait_ld();
+        float o[32];
+#pragma unroll
+        for (int q = 0; q < 32; ++q) o[q] = __uint_as_float(u[q]);
+        if (it.alt) {
+          tmem_ld32(tO + 128 + c4 * 32, u);
+          tmem_wait_ld();
+#pragma unroll
+          for (int q = 0; q < 32; ++q) o[q] = o[q] * a0 + __uint_as_float(u[q]) * a1;
+        }
+        if (any_bad != 0 && valid) {
+          for (int w = 0; w < bad_n; ++w) {
+            for (unsigned b = bad[w]; b != 0; b &= b - 1) {
+              const int k = (it.t0 + dirty) * 128 + w * 32 + __ffs(b) - 1;
+              if (!row_sees<TREE>(it, mask, p.words, token, k)) continue;
+              const uint16_t* vr = value_row<TREE>(p, it, D, k);
+              if (vr == nullptr) continue;
+              vr += c4 * 32;
+#pragma unroll
+              for (int q = 0; q < 32; ++q)
+                if (nonfinite16<F16>(vr[q])) o[q] += widen16<F16>(vr[q]);
+            }
+          }
+        }
+        if (valid) {
+          if (it.part >= 0) {
+            float* w = p.ws_o + (static_cast<long long>(it.part) * 256 + q_tile * 128 + r) * 128 +
+                       c4 * 32;
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              reinterpret_cast<float4*>(w)[q] =
+                  make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+          } else {
+            uint16_t* w = static_cast<uint16_t*>(p.out) + row * p.ldo +
+                          static_cast<long long>(head) * D + c4 * 32;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint4 v;
+              v.x = pack16<F16>(o[8 * q] * inv, o[8 * q + 1] * inv);
+              v.y = pack16<F16>(o[8 * q + 2] * inv, o[8 * q + 3] * inv);
+              v.z = pack16<F16>(o[8 * q + 4] * inv, o[8 * q + 5] * inv);
+              v.w = pack16<F16>(o[8 * q + 6] * inv, o[8 * q + 7] * inv);
+              reinterpret_cast<uint4*>(w)[q] = v;
+            }
+          }
+        }
+      }
+      if (it.part >= 0 && valid)
+        reinterpret_cast<float2*>(p.ws_ml)[static_cast<long long>(it.part) * 256 + q_tile * 128 +
+                                           r] = make_float2(ml, l);
+      tc_fence_before();
+      mbar_arrive(&o_free[x]);
+      if (it.alt) mbar_arrive(&o_free[1]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bad_free[ord % kRowBadBufs]);
+    }
+  }
+
+  __syncthreads();
+  if (*abort_flag) {
+    // Let copies already in flight land before the CTA exits.
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 1000000ull) __nanosleep(1000);
+    if (threadIdx.x == 0) atomicOr(p.status, kDevWaitTimeout);
+  }
+  if (warp == 8) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Before a kernel's launch: its shared memory, and that it was built with the
+// registers its warps hand over to one another (setmaxnreg draws on those of
+// the launch, and a share that is not there is waited for without end).
+template <typename Kern>
+int row_kernel_ready(Kern* kern, size_t smem) {
+  KVM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+  cudaFuncAttributes a;
+  KVM_CUDA_TRY(cudaFuncGetAttributes(&a, kern));
+  if (a.numRegs * kRowThreads < 256 * kRowSoftmaxRegs + 128 * kRowControlRegs)
+    return fail(KVM_ERR_UNSUPPORTED, "attention kernel built with too few registers");
+  return KVM_OK;
+}
+
+}  // namespace kvm

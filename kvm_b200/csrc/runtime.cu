@@ -109,6 +109,29 @@ int encode_tmap_2d(CUtensorMap* map, const void* base, uint64_t inner,
   return KVM_OK;
 }
 
+int encode_tmap_3d(CUtensorMap* map, const void* base, const uint64_t (&extent)[3],
+                   const uint64_t (&stride_bytes)[2], const uint32_t (&box)[3],
+                   CUtensorMapDataType elem, CUtensorMapSwizzle swizzle) {
+  auto fn = encode_fn();
+  if (!fn) return fail(KVM_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  if (!aligned16(base) || (stride_bytes[0] & 15u) != 0 || (stride_bytes[1] & 15u) != 0)
+    return fail(KVM_ERR_INVALID_ARG,
+                "TMA operand must be 16-byte aligned with strides that are "
+                "multiples of 16 bytes");
+  cuuint64_t dims[3] = {extent[0], extent[1], extent[2]};
+  cuuint64_t strides[2] = {stride_bytes[0], stride_bytes[1]};
+  cuuint32_t boxes[3] = {box[0], box[1], box[2]};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, elem, 3, const_cast<void*>(base), dims, strides, boxes, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(KVM_ERR_CUDA,
+                "cuTensorMapEncodeTiled failed with CUresult " +
+                    std::to_string(static_cast<int>(r)));
+  return KVM_OK;
+}
+
 }  // namespace kvm
 
 namespace kvm {

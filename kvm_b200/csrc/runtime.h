@@ -77,6 +77,11 @@ int encode_tmap_2d(CUtensorMap* map, const void* base, uint64_t inner,
                    uint32_t box_outer, CUtensorMapDataType elem,
                    CUtensorMapSwizzle swizzle);
 
+// The same for a 3-D tensor: strides of the two outer dimensions in bytes.
+int encode_tmap_3d(CUtensorMap* map, const void* base, const uint64_t (&extent)[3],
+                   const uint64_t (&stride_bytes)[2], const uint32_t (&box)[3],
+                   CUtensorMapDataType elem, CUtensorMapSwizzle swizzle);
+
 inline bool aligned16(const void* p) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
 }

@@ -35,6 +35,22 @@ def kv_strides(layout: str, pages: int, layers: int, block_size: int, width: int
     return page, layer, kv, width
 
 
+def tree_mask(parents, device=None) -> torch.Tensor:
+    """The masks of a drafted tree for `tree_decode`: parents[i] is the index of
+    node i's parent (below i), or -1 for a child of the last cached token. Row
+    i has the bits of i and of its ancestors: int32 [len(parents), words]."""
+    rows = []
+    for i, p in enumerate(int(p) for p in parents):
+        if not -1 <= p < i:
+            raise ValueError(f"parents[{i}] must be -1 or the index of an earlier node")
+        rows.append((rows[p] if p >= 0 else 0) | (1 << i))
+    words = max(1, (len(rows) + 31) // 32)
+    data = b"".join(r.to_bytes(4 * words, "little") for r in rows)
+    t = torch.frombuffer(bytearray(data), dtype=torch.int32) if rows else \
+        torch.empty(0, dtype=torch.int32)
+    return t.view(len(rows), words).to(device)
+
+
 class PagedKVCache:
     """A device pool of KV pages (bf16, zero-initialised)."""
 
@@ -100,6 +116,59 @@ class PagedKVCache:
              q_offsets.data_ptr(), q_positions.data_ptr(), block_table.data_ptr(),
              bt_offsets.data_ptr(), S, heads_q, max_q_rows, max_keys, float(scale),
              workspace.data_ptr(), workspace.numel(), _stream())
+        return out
+
+    def tree_workspace(self, sequences: int, *, heads_q: int, max_q_rows: int,
+                       max_keys: int) -> int:
+        """Bytes of workspace `tree_decode` needs for these bounds."""
+        return int(_lib.lib().kvm_sm100_attention_tree_workspace(
+            sequences, heads_q, self.heads_kv, max_q_rows, max_keys))
+
+    def tree_decode(self, layer: int, q: torch.Tensor, q_offsets: torch.Tensor,
+                    q_positions: torch.Tensor, tree_mask: torch.Tensor,
+                    block_table: torch.Tensor, bt_offsets: torch.Tensor, *, heads_q: int,
+                    max_q_rows: int, max_keys: int, scale: float = 0.0,
+                    out: torch.Tensor | None = None,
+                    workspace: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of trees of drafted tokens q [rows, HQ*128], written with
+        `write` at positions q_positions[s] + i: row i of sequence s attends to
+        the q_positions[s] tokens before the tree and to the drafted tokens
+        named by its tree_mask row (int32 [rows, words], bit j % 32 of word
+        j / 32 for token j; see tree_mask()). A row that sees nothing is zero.
+        Two calls that overlap in time need a workspace each."""
+        _check(q, "q", torch.bfloat16, 2)
+        _check(tree_mask, "tree_mask", torch.int32, 2)
+        for t, n in ((q_offsets, "q_offsets"), (q_positions, "q_positions"),
+                     (block_table, "block_table"), (bt_offsets, "bt_offsets")):
+            self._index(t, n)
+        S, dev = q_positions.numel(), self.pool.device
+        if q_offsets.numel() != S + 1 or bt_offsets.numel() != S + 1:
+            raise ValueError("q_offsets and bt_offsets must have one more entry than "
+                             "q_positions")
+        if q.device != dev or q.shape[1] != heads_q * 128:
+            raise ValueError(f"q must be [rows, {heads_q} * 128] on the pool's device")
+        if tree_mask.shape[0] != q.shape[0] or not tree_mask.is_contiguous() or \
+                tree_mask.device != dev:
+            raise ValueError("tree_mask must be contiguous [rows, words] on the pool's device")
+        if out is None:
+            out = torch.zeros(q.shape, dtype=q.dtype, device=dev)
+        _check(out, "out", torch.bfloat16, 2)
+        if out.shape != q.shape or out.device != dev:
+            raise ValueError("out must have q's shape and device")
+        if workspace is None:
+            need = self.tree_workspace(S, heads_q=heads_q, max_q_rows=max_q_rows,
+                                       max_keys=max_keys)
+            workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        elif workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous on the pool's device")
+        with torch.cuda.device(dev):
+            call("kvm_sm100_attention_tree_paged", q.data_ptr(), _rowmajor(q, "q"),
+                 self.pool.data_ptr(), C.byref(self.layout_struct(layer)), out.data_ptr(),
+                 _rowmajor(out, "out"), q_offsets.data_ptr(), q_positions.data_ptr(),
+                 tree_mask.data_ptr(), tree_mask.shape[1], block_table.data_ptr(),
+                 bt_offsets.data_ptr(), S, q.shape[0], heads_q, max_q_rows, max_keys,
+                 float(scale), workspace.data_ptr(),
+                 workspace.numel() * workspace.element_size(), _stream())
         return out
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:

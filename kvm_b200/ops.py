@@ -236,6 +236,42 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, batc
     return out
 
 
+_ATTN_DTYPE = {torch.bfloat16: _lib.EW_DTYPES["bf16"], torch.float16: _lib.EW_DTYPES["f16"]}
+
+
+def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                     offsets: torch.Tensor, *, heads_q: int, heads_kv: int,
+                     head_dim: int = 128, scale: float = 0.0,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal GQA attention over packed sequences of different lengths.
+
+    q [rows, HQ*head_dim], k/v [rows, HKV*head_dim] (bf16 or fp16, row views
+    ok); offsets: int32 [S+1] on the device, sequence s owns rows
+    offsets[s]:offsets[s+1] (it may be empty). head_dim 64 or 128. Rows that
+    belong to no sequence are not written (a new `out` starts as zeros).
+    """
+    if not isinstance(q, torch.Tensor) or q.dtype not in _ATTN_DTYPE:
+        raise TypeError("q must be a bf16 or fp16 tensor")
+    for t, n, h in ((q, "q", heads_q), (k, "k", heads_kv), (v, "v", heads_kv)):
+        _check(t, n, q.dtype, 2)
+        if t.shape != (q.shape[0], h * head_dim) or t.device != q.device:
+            raise ValueError(f"{n} must be [{q.shape[0]}, {h} * {head_dim}] on q's device")
+    _check(offsets, "offsets", torch.int32, 1)
+    if offsets.numel() < 1 or not offsets.is_contiguous() or offsets.device != q.device:
+        raise ValueError("offsets must be contiguous [S+1] on q's device")
+    if out is None:
+        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    _check(out, "out", q.dtype, 2)
+    if out.shape != q.shape or out.device != q.device:
+        raise ValueError("out must have q's shape and device")
+    with torch.cuda.device(q.device):
+        call("kvm_sm100_attention_packed", q.data_ptr(), _rowmajor(q, "q"), k.data_ptr(),
+             _rowmajor(k, "k"), v.data_ptr(), _rowmajor(v, "v"), out.data_ptr(),
+             _rowmajor(out, "out"), offsets.data_ptr(), offsets.numel() - 1, q.shape[0],
+             heads_q, heads_kv, head_dim, _ATTN_DTYPE[q.dtype], float(scale), _stream())
+    return out
+
+
 def rope_(x: torch.Tensor, *, seq_len: int, heads: int, head_dim: int = 128,
           base: float = 10000.0) -> torch.Tensor:
     """In-place rotary embedding of x [B*L, >= heads*head_dim] (a row view is ok)."""
@@ -512,7 +548,7 @@ def device_status() -> int:
 
 __all__ = [
     "matmul", "gemm", "pack_gate_up", "quantize_e4m3", "matmul_fp8", "transpose_u8",
-    "transpose_f32", "attention_prefill", "rope_", "rope_table", "rope", "transpose", "silu_gate_matmul", "rmsnorm",
+    "transpose_f32", "attention_prefill", "attention_packed", "rope_", "rope_table", "rope", "transpose", "silu_gate_matmul", "rmsnorm",
     "silu_mul", "moe_route", "moe_permute", "moe_scatter_rows", "grouped_matmul",
     "moe_combine", "Routing", "Dispatch", "elementwise", "device_status", "KVM_B_KN", "KVM_B_NK",
 ]

@@ -128,3 +128,63 @@ def test_page_calls_refuse_without_a_gpu():
     assert comp(P, C.byref(L), 1, P, -1, P, P, P, P, 1, None) == INV
     assert comp(P + 8, C.byref(L), 1, P, 1, P, P, P, P, 1, None) == INV
     assert comp(P, C.byref(L), 1, None, 0, None, None, None, None, 1, None) == _lib.KVM_OK
+
+
+def test_tree_mask():
+    from kvm_b200.kvcache import tree_mask
+    m = tree_mask([-1, 0, 0, 1, -1])
+    assert m.tolist() == [[1], [3], [5], [11], [16]]
+    chain = tree_mask(range(-1, 69))
+    assert chain.shape == (70, 3)
+    got = [sum((w & 0xFFFFFFFF) << (32 * i) for i, w in enumerate(r)) for r in chain.tolist()]
+    assert got == [(1 << (i + 1)) - 1 for i in range(70)]
+    assert tree_mask([]).shape == (0, 1)
+    for bad in ([0], [-1, 1], [-1, -2], [-1, 5]):
+        with pytest.raises(ValueError):
+            tree_mask(bad)
+
+
+def test_attention_packed_refuses_without_a_gpu():
+    P, INV, UNS = 4096, _lib.KVM_ERR_INVALID_ARG, _lib.KVM_ERR_UNSUPPORTED
+    ok = [P, 512, P, 256, P, 256, P, 512, P, 3, 100, 4, 2, 128, 0, 0.0, None]
+
+    def rc(**at):
+        args = list(ok)
+        for i, v in at.items():
+            args[int(i[1:])] = v
+        return _rc("attention_packed", *args)
+    assert rc(a9=-1) == INV and rc(a10=-1) == INV and rc(a11=3) == INV and rc(a12=0) == INV
+    assert rc(a13=32) == UNS and rc(a14=1) == UNS and rc(a9=1025) == UNS
+    assert rc(a11=258, a1=1 << 20, a7=1 << 20) == UNS       # 129 query heads a kv head
+    assert rc(a15=float("inf")) == INV
+    assert rc(a0=None) == INV and rc(a4=P + 2) == INV and rc(a8=None) == INV
+    assert rc(a1=504) == INV and rc(a3=260) == INV and rc(a7=500) == INV
+    assert rc(a9=0) == _lib.KVM_OK and rc(a10=0) == _lib.KVM_OK
+
+
+def test_attention_tree_refuses_without_a_gpu():
+    P, INV, UNS = 4096, _lib.KVM_ERR_INVALID_ARG, _lib.KVM_ERR_UNSUPPORTED
+    lay = dict(page_stride=8192, layer_stride=8192, kv_stride=4096, token_stride=256,
+               block_size=16, layer=0, width=256, num_pages=9)
+
+    def rc(layout=None, **at):
+        L = _lib.KvLayout(*{**lay, **(layout or {})}.values())
+        args = [P, 1024, P, C.byref(L), P, 1024, P, P, P, 1, P, P, 2, 10, 8, 5, 100, 0.0, P,
+                1 << 40, None]
+        for i, v in at.items():
+            args[int(i[1:])] = v
+        return _rc("attention_tree_paged", *args)
+    assert rc(a3=None) == INV and rc(layout=dict(width=192)) == INV and rc(a14=7) == INV
+    assert rc(layout=dict(block_size=8)) == UNS and rc(layout=dict(block_size=48)) == UNS
+    assert rc(layout=dict(kv_stride=4096 + 8)) == INV
+    assert rc(a12=1025) == UNS and rc(a15=0) == INV and rc(a15=1025, a9=64) == INV
+    assert rc(a15=33) == INV and rc(a16=0) == INV and rc(a17=float("nan")) == INV
+    assert rc(a0=None) == INV and rc(a4=P + 4) == INV and rc(a8=None) == INV and rc(a1=1000) == INV
+    assert rc(a18=None) == INV and rc(a19=100) == INV
+    assert rc(layout=dict(num_pages=1 << 30, page_stride=1 << 20)) == UNS
+    assert rc(a12=0) == _lib.KVM_OK and rc(a13=0) == _lib.KVM_OK
+    ws = _lib.lib().kvm_sm100_attention_tree_workspace
+    assert ws(0, 8, 2, 5, 100) == 0 and ws(2, 7, 2, 5, 100) == 0 and ws(2, 8, 2, 0, 100) == 0
+    # one stretch for the two sequences' four one-tile items
+    assert ws(2, 8, 2, 5, 100) == 2 * 256 * 130 * 4
+    assert ws(64, 64, 8, 16, 5000) == 148 * 2 * 256 * 130 * 4
