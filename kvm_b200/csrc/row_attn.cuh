@@ -12,21 +12,21 @@
 //                    from TMEM to registers, mask, running max m and sum l,
 //                    P = 2^(s - m) rounded to the input type over S's own
 //                    columns in TMEM; at the end O / l to global memory
-//   warp 8 (1 lane)  MMA issuer: S_x = Q_x K_j^T (shared memory operands),
-//                    O_x += P_x V_j (P from TMEM: shared memory carries Q, K
-//                    and V reads only, 96 bytes a clock at full MMA rate
-//                    instead of 160)
-//   warp 9           TMA producer of the K and V tiles (one ring for both)
-//   warp 10 (1 lane) TMA producer of the Q tiles
-//   warp 11          looks over each V tile that some row must not see whole
+//   warps 8, 9       MMA issuer (one lane) of stream 0 and 1: S_x = Q_x K_j^T
+//                    (shared memory operands), O_x += P_x V_j (P from TMEM:
+//                    shared memory carries Q, K and V reads only, 96 bytes a
+//                    clock at full MMA rate instead of 160)
+//   warp 10          TMA producer of the K and V tiles (one ring for both)
+//   warp 11 (1 lane) TMA producer of the Q tiles
+//   warp 12          looks over each V tile that some row must not see whole
 //
 // Two streams keep the tensor cores fed: while one does its softmax, the
 // other's P V and next Q K^T run. In PAIR items the streams are two Q tiles
 // that read the same K/V tiles. An item with one Q tile runs as ALT: both
 // streams hold that tile and take the even and the odd key tiles, and stream
-// 0 merges the two results at the end. The issuer walks the streams through
-// the items independently, so the next item's first S is computed while the
-// other stream still finishes this one.
+// 0 merges the two results at the end. Each stream has its own issuing warp:
+// with one thread issuing for both, its waits and commits (2000 cycles a
+// step) came between the products (16383 tokens of 32 + 4 heads: 2.97 ms).
 //
 // P overwrites S in place, so S_x(j+1) is issued after P V_x(j): MMAs of one
 // thread execute in order. For the same reason S_x(j+1) being complete means
@@ -54,10 +54,10 @@
 
 namespace kvm {
 
-constexpr int kRowThreads = 384;
-// Registers a thread after the warps have split up: 168 * 384 at launch.
-constexpr int kRowSoftmaxRegs = 216;    // warps 0-7
-constexpr int kRowControlRegs = 72;     // warps 8-11
+constexpr int kRowThreads = 512;
+// Registers a thread after the warps have split up: 128 * 512 at launch.
+constexpr int kRowSoftmaxRegs = 200;    // warps 0-7
+constexpr int kRowControlRegs = 56;     // warps 8-15
 constexpr float kRowRescale = 8.0f;     // log2 units
 constexpr int kRowMaxSeqs = 1024;       // sequences of one call (tables in shared memory)
 constexpr int kRowMaxDirty = 10;        // V tiles of an item that a row sees in part
@@ -80,9 +80,9 @@ struct RowSmem {
   static constexpr uint32_t kOffPages = kOffMl + 2 * 128 * 8;
   static constexpr uint32_t kPageSlots = 128;                // page ids read ahead
   static constexpr uint32_t kOffBar = kOffPages + kPageSlots * 4;
-  // q_full[2] q_empty[2] kv_full[S] kv_empty[S] v_ok[S] s_full[2] p_full[2]
+  // q_full[2] q_empty[2] kv_full[S] kv_empty[S] s_full[2] p_full[2]
   // o_full[2] o_free[2] alt_ml[2] looked[8] bad_free[8] drain
-  static constexpr int kBars = 3 * kStages + 14 + 2 * kRowBadBufs + 1;
+  static constexpr int kBars = 2 * kStages + 14 + 2 * kRowBadBufs + 2;
   static constexpr size_t bytes() { return 1024 + kOffBar + kBars * 8 + 16; }
 };
 
@@ -341,6 +341,65 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
       : "memory");
 }
 
+// A count in shared memory that one warp raises and others wait for.
+__device__ __forceinline__ void st_release_cta(uint32_t* p, uint32_t v) {
+  asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_acquire_cta(const uint32_t* p) {
+  uint32_t v;
+  asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory");
+  return v;
+}
+__device__ __forceinline__ bool count_wait(const uint32_t* p, uint32_t at_least,
+                                           volatile int* abort) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 0;; ++i) {
+    if (static_cast<int32_t>(ld_acquire_cta(p) - at_least) >= 0) return true;
+    if ((i & 255u) == 255u) {
+      if (*abort) return false;
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) {
+        t0 = now;
+      } else if (now - t0 > kWaitTimeoutNs) {
+        *abort = 1;
+        return false;
+      }
+    }
+  }
+}
+
+// A lock in shared memory between two threads of the CTA that each hold it
+// for a bounded time. Returns false when the wait gave up.
+__device__ __forceinline__ bool lock_take(uint32_t* p, volatile int* abort) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 0;; ++i) {
+    uint32_t was;
+    asm volatile("atom.acquire.cta.shared::cta.cas.b32 %0, [%1], 0, 1;"
+                 : "=r"(was) : "r"(smem_u32(p)) : "memory");
+    if (was == 0) return true;
+    if ((i & 255u) == 255u) {
+      if (*abort) return false;
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) {
+        t0 = now;
+      } else if (now - t0 > kWaitTimeoutNs) {
+        *abort = 1;
+        return false;
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+
 // 3-D tiled TMA load (x innermost).
 __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, uint64_t* bar,
                                             int32_t x, int32_t y, int32_t z) {
@@ -349,6 +408,13 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, uint64_
       "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
       "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
+}
+
+// max of three, NaN ignored as by fmaxf.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 template <int N>
@@ -453,17 +519,18 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   uint64_t* q_empty = q_full + 2;               // [2]
   uint64_t* kv_full = q_empty + 2;              // [NST]
   uint64_t* kv_empty = kv_full + NST;           // [NST]
-  uint64_t* v_ok = kv_empty + NST;              // [NST] 32 arrivals
-  uint64_t* s_full = v_ok + NST;                // [2]
+  uint64_t* s_full = kv_empty + NST;            // [2]
   uint64_t* p_full = s_full + 2;                // [2] 128 arrivals
   uint64_t* o_full = p_full + 2;                // [2]
   uint64_t* o_free = o_full + 2;                // [2] 128 arrivals
   uint64_t* alt_ml = o_free + 2;                // [2] 128 arrivals
   uint64_t* looked = alt_ml + 2;                // [kRowBadBufs] 32 arrivals
   uint64_t* bad_free = looked + kRowBadBufs;    // [kRowBadBufs] 8 arrivals
-  uint64_t* drain = bad_free + kRowBadBufs;
+  uint64_t* drain = bad_free + kRowBadBufs;     // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint32_t* v_count = tmem_slot + 2;            // V tiles looked over, ever
+  uint32_t* mma_lock = tmem_slot + 3;
   unsigned* bad_words = reinterpret_cast<unsigned*>(smem + L::kOffBad);
   float2* alt_buf = reinterpret_cast<float2*>(smem + L::kOffMl);   // [2][128]
   const RowTables tab = row_tables<D>(smem);
@@ -473,9 +540,12 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
+    *v_count = 0;
+    *mma_lock = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 2 - i);
+      mbar_init(&drain[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 128);
       mbar_init(&o_full[i], 1);
@@ -485,13 +555,11 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     for (int i = 0; i < NST; ++i) {
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 2);
-      mbar_init(&v_ok[i], 32);
     }
     for (int i = 0; i < kRowBadBufs; ++i) {
       mbar_init(&looked[i], 32);
       mbar_init(&bad_free[i], 8);
     }
-    mbar_init(drain, 1);
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
@@ -512,7 +580,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 
   if (warp >= 8) {
     reg_give<kRowControlRegs>();
-    if (warp == 9) {
+    if (warp == 10) {
       // ------------------------------------------------ K/V producer
       int* page_ids = reinterpret_cast<int*>(smem + L::kOffPages);
       Items items;
@@ -588,7 +656,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         }
         __syncwarp();
       }
-    } else if (warp == 10) {
+    } else if (warp == 11) {
       if (lane == 0) {
         // ---------------------------------------------- Q producer
         Items items;
@@ -609,7 +677,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           }
         }
       }
-    } else if (warp == 11) {
+    } else if (warp == 12) {
       // ------------------------------------------------ value tiles
       Items items;
       RowItem it;
@@ -663,136 +731,103 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             }
             fence_async_smem();
           }
-          mbar_arrive(&v_ok[st]);
+          __syncwarp();
+          if (lane == 0) st_release_cta(v_count, c + 1);
         }
         if (!ok) break;
         mbar_arrive(&looked[ord % kRowBadBufs]);
         ++ord;
       }
-    } else if (lane == 0) {
+    } else if (warp < 10 && lane == 0) {
       // ------------------------------------------------ MMA issuer
       constexpr uint32_t kIdescQK = row_idesc<F16>(128, 0);
       constexpr uint32_t kIdescPV = row_idesc<F16>(D, 1);
-      // Each stream has a cursor: the key tile it is at, and whether S or P V
-      // comes next there.
-      struct Cursor {
-        Items items;
-        RowItem it;
-        bool live, scored;   // scored: S of the tile is issued, P V comes next
-        int i, cnt;          // position in the stream's tiles of the item
-        uint32_t base;       // key tiles of the items before
-        uint32_t ord0, ord1; // items so far that used Q tile 0 (all) / 1
-        uint32_t tiles;      // tiles of the stream so far
-        uint32_t mine;       // items of the stream so far
-      };
-      Cursor cur[2];
+      const int x = warp - 8;
+      const uint32_t tS = tmem + x * 128, tO = tmem + 256 + x * 128;
+      Items items;
+      RowItem it;
+      uint32_t base = 0;          // key tiles of the items before
+      uint32_t ord0 = 0, ord1 = 0;  // items before; those with a Q tile 1
+      uint32_t tiles = 0, mine = 0;  // tiles and items of the stream before
       bool ok = true;
-      // The stream's next item with work for it.
-      auto advance = [&](Cursor& c, int x, bool begin) {
-        for (;;) {
-          if (!begin) {
-            c.base += c.it.n;
-            ++c.ord0;
-            c.ord1 += c.it.n1 > 0;
+      for (; ok && items.next(p, tab, it); base += it.n, ++ord0, ord1 += it.n1 > 0) {
+        const int cnt = it.count(x);
+        const int qt = it.alt ? 0 : x;
+        // Both streams look at Q tile 0 of every item, and both give it back:
+        // neither can be a phase of any barrier ahead of the other's items.
+        if (!mbar_wait(&q_full[0], ord0 & 1, abort_flag)) break;
+        if (x == 1 && !it.alt) mbar_arrive(&q_empty[0]);
+        const uint64_t q_desc = sdesc_sw128(smem_u32(smem + L::kOffQ + qt * L::kTile), 0, 1024);
+        auto k_ready = [&](int i) {
+          const uint32_t slot = 2 * (base + it.tile(x, i));
+          return mbar_test(&kv_full[slot % NST], (slot / NST) & 1);
+        };
+        // K of the stream's i-th tile (and its Q tile) are in shared memory.
+        auto wait_k = [&](int i) {
+          const uint32_t slot = 2 * (base + it.tile(x, i));
+          return (i > 0 || !qt || mbar_wait(&q_full[1], ord1 & 1, abort_flag)) &&
+                 mbar_wait(&kv_full[slot % NST], (slot / NST) & 1, abort_flag);
+        };
+        auto issue_s = [&](int i) {
+          const int j = it.tile(x, i);
+          const uint32_t st = 2 * (base + j) % NST;
+          const uint64_t k_desc = sdesc_sw128(smem_u32(smem + L::kOffKV + st * L::kTile), 0, 1024);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = ((kk >> 2) * L::kHalf + (kk & 3) * 32) >> 4;
+            mma_f16_ss(tS, q_desc + off, k_desc + off, kIdescQK, kk > 0);
           }
-          begin = false;
-          c.live = c.items.next(p, tab, c.it);
-          if (!c.live) return;
-          c.i = 0;
-          c.scored = false;
-          c.cnt = c.it.count(x);
-          if (c.cnt > 0) return;
-        }
-      };
-      // Whether the stream's next step may be waited for with the other stream
-      // where it is. The ring holds kStages / 2 >= 2 key tiles and is filled in
-      // order: K of tile g needs every S up to g - 2 and every P V up to g - 3
-      // issued, V of tile g every P V up to g - 2. An item's Q tiles are loaded
-      // once every S of the items before is issued. The first P V of an item
-      // waits for the epilogue of the one before, which in an ALT item needs
-      // both streams' P V. The stream that is behind may always go on.
-      auto may = [&](const Cursor& c, int x, const Cursor& o, int ox) {
-        if (!o.live) return true;
-        const int g = c.base + c.it.tile(x, c.i), og = o.base + o.it.tile(ox, o.i);
-        if (!c.scored)
-          return og >= g - (o.scored ? 2 : 1) &&
-                 (c.i > 0 || o.ord0 >= c.ord0 ||
-                  (o.ord0 + 1 == c.ord0 && o.scored && o.i == o.cnt - 1));
-        return og >= g - 1 && (c.i > 0 || o.ord0 >= c.ord0);
-      };
-      auto issue_s = [&](Cursor& c, int x) {
-        const int j = c.it.tile(x, c.i);
-        const int qt = c.it.alt ? 0 : x;
-        const uint32_t slot = 2 * (c.base + j), st = slot % NST;
-        if ((c.i == 0 && !mbar_wait(&q_full[qt], (qt ? c.ord1 : c.ord0) & 1, abort_flag)) ||
-            !mbar_wait(&kv_full[st], (slot / NST) & 1, abort_flag)) {
-          ok = false;
-          return;
-        }
+          mma_commit(&s_full[x]);
+          // Two arrivals free a slot: one of each stream, or both of its only one.
+          mma_commit(&kv_empty[st]);
+          if (!it.shared(j)) mma_commit(&kv_empty[st]);
+          if (i == cnt - 1) mma_commit(&q_empty[qt]);
+        };
+        if (cnt == 0) continue;
+        if (!wait_k(0) || !lock_take(mma_lock, abort_flag)) break;
         tc_fence_after();
-        const uint32_t q_addr = smem_u32(smem + L::kOffQ + qt * L::kTile);
-        const uint32_t k_addr = smem_u32(smem + L::kOffKV + st * L::kTile);
+        issue_s(0);
+        st_release_cta(mma_lock, 0);
+        for (int i = 0; i < cnt; ++i) {
+          const int j = it.tile(x, i);
+          const uint32_t st = (2 * (base + j) + 1) % NST;
+          if (!count_wait(v_count, base + j + 1, abort_flag) ||
+              (i == 0 && !mbar_wait(&o_free[x], (mine & 1) ^ 1, abort_flag)) ||
+              !mbar_wait(&p_full[x], tiles & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const bool both = i + 1 < cnt && k_ready(i + 1);
+          if (!lock_take(mma_lock, abort_flag)) { ok = false; break; }
+          // P V of this tile and S of the next go out together: the streams'
+          // products then follow one another, and one's softmax runs under the
+          // other's products, instead of both at half speed side by side.
+          ++tiles;
+          tc_fence_after();
+          const uint64_t v_desc =
+              sdesc_sw128(smem_u32(smem + L::kOffKV + st * L::kTile), L::kHalf, 1024);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * L::kHalf + (kk & 3) * 32;
-          mma_f16_ss(tmem + x * 128, sdesc_sw128(q_addr + off, 0, 1024),
-                     sdesc_sw128(k_addr + off, 0, 1024), kIdescQK, kk > 0);
+          for (int kk = 0; kk < 8; ++kk)
+            mma_f16_ts(tO, tS + kk * 8, v_desc + kk * (2048 >> 4), kIdescPV,
+                       (i > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(&kv_empty[st]);
+          if (!it.shared(j)) mma_commit(&kv_empty[st]);
+          if (i == cnt - 1) mma_commit(&o_full[x]);
+          if (both) issue_s(i + 1);
+          st_release_cta(mma_lock, 0);
+          if (i + 1 < cnt && !both) {
+            if (!wait_k(i + 1) || !lock_take(mma_lock, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            issue_s(i + 1);
+            st_release_cta(mma_lock, 0);
+          }
         }
-        mma_commit(&s_full[x]);
-        // Two arrivals free a slot: one of each stream, or both of its only one.
-        mma_commit(&kv_empty[st]);
-        if (!c.it.shared(j)) mma_commit(&kv_empty[st]);
-        if (c.i == c.cnt - 1) {
-          mma_commit(&q_empty[qt]);
-          if (qt == 0 && !c.it.alt) mma_commit(&q_empty[0]);
-        }
-        c.scored = true;
-      };
-      auto issue_pv = [&](Cursor& c, int x) {
-        const int j = c.it.tile(x, c.i);
-        const uint32_t slot = 2 * (c.base + j) + 1, st = slot % NST;
-        if (!mbar_wait(&p_full[x], c.tiles & 1, abort_flag) ||
-            (c.i == 0 && !mbar_wait(&o_free[x], (c.mine & 1) ^ 1, abort_flag)) ||
-            !mbar_wait(&kv_full[st], (slot / NST) & 1, abort_flag) ||
-            !mbar_wait(&v_ok[st], (slot / NST) & 1, abort_flag)) {
-          ok = false;
-          return;
-        }
-        tc_fence_after();
-        const uint32_t v_addr = smem_u32(smem + L::kOffKV + st * L::kTile);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          mma_f16_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8,
-                     sdesc_sw128(v_addr + kk * 2048, L::kHalf, 1024), kIdescPV,
-                     (c.i > 0 || kk > 0) ? 1u : 0u);
-        mma_commit(&kv_empty[st]);
-        if (!c.it.shared(j)) mma_commit(&kv_empty[st]);
-        if (c.i == c.cnt - 1) mma_commit(&o_full[x]);
-        ++c.tiles;
-        c.scored = false;
-        if (++c.i == c.cnt) {
-          ++c.mine;
-          advance(c, x, false);
-        }
-      };
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        cur[x].base = cur[x].ord0 = cur[x].ord1 = cur[x].tiles = cur[x].mine = 0;
-        advance(cur[x], x, true);
-      }
-      while (ok && (cur[0].live || cur[1].live)) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          Cursor& c = cur[x];
-          const Cursor& o = cur[1 - x];
-          if (ok && c.live && c.scored && may(c, x, o, 1 - x)) issue_pv(c, x);
-          if (ok && c.live && !c.scored && may(c, x, o, 1 - x)) issue_s(c, x);
-        }
+        ++mine;
       }
       // Every MMA issued above must finish before TMEM is released.
-      mma_commit(drain);
+      mma_commit(&drain[x]);
       volatile int local_abort = 0;
-      mbar_wait(drain, 0, &local_abort);
+      mbar_wait(&drain[x], 0, &local_abort);
     }
   } else {
     // ------------------------------------------------ softmax / epilogue
@@ -854,13 +889,15 @@ __global__ void __launch_bounds__(kRowThreads, 1)
               if (c > lim) s[c] = -INFINITY;
           }
         }
-        // Row max as four chains (max is exact in any order).
+        // Row max as four chains (max is exact in any order), two values a step.
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int c = 4; c < 128; c += 4)
+        for (int c = 4; c < 124; c += 8)
 #pragma unroll
-          for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], s[c + u]);
-        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          for (int u = 0; u < 4; ++u) mx[u] = max3(mx[u], s[c + u], s[c + 4 + u]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], s[124 + u]);
+        const float mt = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
         if (i == 0) {
           m = mt;
           msl = m == -INFINITY ? 0.f : m * sl2;
@@ -920,8 +957,9 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       float a0 = 1.f, a1 = 0.f;                  // weights of the two streams' O
       float ml = m == -INFINITY ? m : msl;       // running max, log2 units
       if (it.alt) {
-        fin = fin && mbar_wait(&o_full[1], act1 & 1, abort_flag) &&
-              mbar_wait(&alt_ml[alts & 1], (alts >> 1) & 1, abort_flag);
+        // (stream 1's statistics first: by then its earlier items are through)
+        fin = fin && mbar_wait(&alt_ml[alts & 1], (alts >> 1) & 1, abort_flag) &&
+              mbar_wait(&o_full[1], act1 & 1, abort_flag);
         if (__all_sync(0xffffffffu, fin)) {
           const float2 o = alt_buf[(alts & 1) * 128 + r];
           const float mm = fmaxf(ml, o.x);
@@ -1044,7 +1082,7 @@ int row_kernel_ready(Kern* kern, size_t smem) {
   KVM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
   cudaFuncAttributes a;
   KVM_CUDA_TRY(cudaFuncGetAttributes(&a, kern));
-  if (a.numRegs * kRowThreads < 256 * kRowSoftmaxRegs + 128 * kRowControlRegs)
+  if (a.numRegs * kRowThreads < 256 * kRowSoftmaxRegs + 256 * kRowControlRegs)
     return fail(KVM_ERR_UNSUPPORTED, "attention kernel built with too few registers");
   return KVM_OK;
 }
