@@ -19,6 +19,8 @@
 //   warp 10          TMA producer of the K and V tiles (one ring for both)
 //   warp 11 (1 lane) TMA producer of the Q tiles
 //   warp 12          looks over each V tile that some row must not see whole
+//   warp 13 (1 lane) works out the CTA's next items for the other warps: a ring
+//                    of kRowItems descriptions in shared memory
 //
 // Two streams keep the tensor cores fed: while one does its softmax, the
 // other's P V and next Q K^T run. In PAIR items the streams are two Q tiles
@@ -61,7 +63,8 @@ constexpr int kRowControlRegs = 56;     // warps 8-15
 constexpr float kRowRescale = 8.0f;     // log2 units
 constexpr int kRowMaxSeqs = 1024;       // sequences of one call (tables in shared memory)
 constexpr int kRowMaxDirty = 10;        // V tiles of an item that a row sees in part
-constexpr int kRowBadBufs = 8;          // items whose bad-value lists can be alive
+constexpr int kRowItems = 4;            // item descriptions in the ring
+constexpr int kRowItemUsers = 13;       // warps that give one back: 0-12
 constexpr int kRowMaxNodes = 1024;
 
 // Shared memory of one CTA for head width D.
@@ -76,13 +79,15 @@ struct RowSmem {
   static constexpr uint32_t kOffTab = kOffKV + kStages * kTile;
   static constexpr uint32_t kTabBytes = kRowMaxSeqs * 10 + 16;
   static constexpr uint32_t kOffBad = kOffTab + kTabBytes;
-  static constexpr uint32_t kOffMl = kOffBad + kRowBadBufs * kRowMaxDirty * 16;
+  static constexpr uint32_t kOffItems = kOffBad + kRowItems * kRowMaxDirty * 16;
+  static constexpr uint32_t kOffMl = kOffItems + kRowItems * 64;
   static constexpr uint32_t kOffPages = kOffMl + 2 * 128 * 8;
   static constexpr uint32_t kPageSlots = 128;                // page ids read ahead
-  static constexpr uint32_t kOffBar = kOffPages + kPageSlots * 4;
+  static constexpr uint32_t kOffOut = kOffPages + kPageSlots * 4;  // [8 warps][32 rows][64 B]
+  static constexpr uint32_t kOffBar = kOffOut + 8 * 2048;
   // q_full[2] q_empty[2] kv_full[S] kv_empty[S] s_full[2] p_full[2]
-  // o_full[2] o_free[2] alt_ml[2] looked[8] bad_free[8] drain
-  static constexpr int kBars = 2 * kStages + 14 + 2 * kRowBadBufs + 2;
+  // o_full[2] o_free[2] alt_ml[2] looked[I] it_full[I] it_empty[I] drain[2]
+  static constexpr int kBars = 2 * kStages + 16 + 3 * kRowItems;
   static constexpr size_t bytes() { return 1024 + kOffBar + kBars * 8 + 16; }
 };
 
@@ -410,10 +415,15 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, uint64_
       : "memory");
 }
 
-// max of three, NaN ignored as by fmaxf.
+// Maxima that are NaN when an argument is: a row that sees a NaN score is NaN.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
@@ -524,9 +534,10 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   uint64_t* o_full = p_full + 2;                // [2]
   uint64_t* o_free = o_full + 2;                // [2] 128 arrivals
   uint64_t* alt_ml = o_free + 2;                // [2] 128 arrivals
-  uint64_t* looked = alt_ml + 2;                // [kRowBadBufs] 32 arrivals
-  uint64_t* bad_free = looked + kRowBadBufs;    // [kRowBadBufs] 8 arrivals
-  uint64_t* drain = bad_free + kRowBadBufs;     // [2]
+  uint64_t* looked = alt_ml + 2;                // [kRowItems]
+  uint64_t* it_full = looked + kRowItems;       // [kRowItems]
+  uint64_t* it_empty = it_full + kRowItems;     // [kRowItems] kRowItemUsers arrivals
+  uint64_t* drain = it_empty + kRowItems;       // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint32_t* v_count = tmem_slot + 2;            // V tiles looked over, ever
@@ -534,6 +545,18 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   unsigned* bad_words = reinterpret_cast<unsigned*>(smem + L::kOffBad);
   float2* alt_buf = reinterpret_cast<float2*>(smem + L::kOffMl);   // [2][128]
   const RowTables tab = row_tables<D>(smem);
+
+  RowItem* ring = reinterpret_cast<RowItem*>(smem + L::kOffItems);
+  static_assert(sizeof(RowItem) == 64, "one 64-byte slot each");
+  // The next item for a warp (or its one lane): the ord-th of the CTA. False
+  // at the end, or when the wait gave up. A slot is given back by every user.
+  auto next_item = [&](uint32_t ord, RowItem& it) {
+    const uint32_t slot = ord % kRowItems;
+    if (!mbar_wait(&it_full[slot], (ord / kRowItems) & 1, abort_flag)) return false;
+    it = ring[slot];
+    return it.n > 0;
+  };
+  auto item_done = [&](uint32_t ord) { mbar_arrive(&it_empty[ord % kRowItems]); };
 
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
@@ -556,9 +579,10 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 2);
     }
-    for (int i = 0; i < kRowBadBufs; ++i) {
-      mbar_init(&looked[i], 32);
-      mbar_init(&bad_free[i], 8);
+    for (int i = 0; i < kRowItems; ++i) {
+      mbar_init(&looked[i], 1);
+      mbar_init(&it_full[i], 1);
+      mbar_init(&it_empty[i], kRowItemUsers);
     }
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -583,11 +607,12 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     if (warp == 10) {
       // ------------------------------------------------ K/V producer
       int* page_ids = reinterpret_cast<int*>(smem + L::kOffPages);
-      Items items;
       RowItem it;
       uint32_t c = 0;  // ring slots filled
       bool ok = true;
-      while (ok && items.next(p, tab, it)) {
+      for (uint32_t ord = 0; ok && __all_sync(0xffffffffu, next_item(ord, it)); ++ord) {
+        __syncwarp();
+        if (lane == 0) item_done(ord);
         int have = -1;  // page ids [have, have + kPageSlots) of the sequence are in shared memory
         for (int j = 0; j < it.n && ok; ++j) {
           const int k0 = (it.t0 + j) * 128;
@@ -659,12 +684,12 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     } else if (warp == 11) {
       if (lane == 0) {
         // ---------------------------------------------- Q producer
-        Items items;
         RowItem it;
         uint32_t uses0 = 0, uses1 = 0;
         const uint32_t bytes = L::kHalves * 64u * 2u * p.group * p.tile_tokens;
         bool ok = true;
-        while (ok && items.next(p, tab, it)) {
+        for (uint32_t ord = 0; ok && next_item(ord, it); ++ord) {
+          item_done(ord);
           for (int x = 0; x < 2 && ok; ++x) {
             if (x == 1 && it.n1 == 0) break;
             uint32_t& uses = x ? uses1 : uses0;
@@ -679,16 +704,12 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       }
     } else if (warp == 12) {
       // ------------------------------------------------ value tiles
-      Items items;
       RowItem it;
-      uint32_t c = 0, ord = 0;
+      uint32_t c = 0;
       bool ok = true;
-      while (ok && items.next(p, tab, it)) {
+      for (uint32_t ord = 0; ok && __all_sync(0xffffffffu, next_item(ord, it)); ++ord) {
         const int dirty = first_dirty<TREE>(it);
-        unsigned* bad = bad_words + (ord % kRowBadBufs) * (kRowMaxDirty * 4);
-        const bool free = mbar_wait(&bad_free[ord % kRowBadBufs],
-                                    ((ord / kRowBadBufs) & 1) ^ 1, abort_flag);
-        if (!__all_sync(0xffffffffu, free)) break;
+        unsigned* bad = bad_words + (ord % kRowItems) * (kRowMaxDirty * 4);
         for (int j = 0; j < it.n; ++j, ++c) {
           const uint32_t slot = 2 * c + 1, st = slot % NST;
           const bool in = mbar_wait(&kv_full[st], (slot / NST) & 1, abort_flag);
@@ -721,6 +742,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                   if ((top & 0xFFFFu) >= inf || (top >> 16) >= inf) {
                     found = true;
                     uint16_t* e = reinterpret_cast<uint16_t*>(row);
+#pragma unroll 1
                     for (int i = 0; i < 64; ++i)
                       if (nonfinite16<F16>(e[i])) e[i] = 0;
                   }
@@ -735,8 +757,26 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           if (lane == 0) st_release_cta(v_count, c + 1);
         }
         if (!ok) break;
-        mbar_arrive(&looked[ord % kRowBadBufs]);
-        ++ord;
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&looked[ord % kRowItems]);
+          item_done(ord);
+        }
+      }
+    } else if (warp == 13) {
+      if (lane == 0) {
+        // ---------------------------------------------- items
+        Items items;
+        RowItem it;
+        for (uint32_t ord = 0;; ++ord) {
+          const uint32_t slot = ord % kRowItems;
+          if (!mbar_wait(&it_empty[slot], ((ord / kRowItems) & 1) ^ 1, abort_flag)) break;
+          const bool more = items.next(p, tab, it);
+          if (!more) it.n = 0;
+          ring[slot] = it;
+          mbar_arrive(&it_full[slot]);
+          if (!more) break;
+        }
       }
     } else if (warp < 10 && lane == 0) {
       // ------------------------------------------------ MMA issuer
@@ -744,13 +784,13 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       constexpr uint32_t kIdescPV = row_idesc<F16>(D, 1);
       const int x = warp - 8;
       const uint32_t tS = tmem + x * 128, tO = tmem + 256 + x * 128;
-      Items items;
       RowItem it;
       uint32_t base = 0;          // key tiles of the items before
       uint32_t ord0 = 0, ord1 = 0;  // items before; those with a Q tile 1
       uint32_t tiles = 0, mine = 0;  // tiles and items of the stream before
       bool ok = true;
-      for (; ok && items.next(p, tab, it); base += it.n, ++ord0, ord1 += it.n1 > 0) {
+      for (; ok && next_item(ord0, it); base += it.n, ++ord0, ord1 += it.n1 > 0) {
+        item_done(ord0);
         const int cnt = it.count(x);
         const int qt = it.alt ? 0 : x;
         // Both streams look at Q tile 0 of every item, and both give it back:
@@ -768,58 +808,61 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           return (i > 0 || !qt || mbar_wait(&q_full[1], ord1 & 1, abort_flag)) &&
                  mbar_wait(&kv_full[slot % NST], (slot / NST) & 1, abort_flag);
         };
-        auto issue_s = [&](int i) {
-          const int j = it.tile(x, i);
-          const uint32_t st = 2 * (base + j) % NST;
-          const uint64_t k_desc = sdesc_sw128(smem_u32(smem + L::kOffKV + st * L::kTile), 0, 1024);
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = ((kk >> 2) * L::kHalf + (kk & 3) * 32) >> 4;
-            mma_f16_ss(tS, q_desc + off, k_desc + off, kIdescQK, kk > 0);
-          }
-          mma_commit(&s_full[x]);
-          // Two arrivals free a slot: one of each stream, or both of its only one.
-          mma_commit(&kv_empty[st]);
-          if (!it.shared(j)) mma_commit(&kv_empty[st]);
-          if (i == cnt - 1) mma_commit(&q_empty[qt]);
-        };
         if (cnt == 0) continue;
-        if (!wait_k(0) || !lock_take(mma_lock, abort_flag)) break;
-        tc_fence_after();
-        issue_s(0);
-        st_release_cta(mma_lock, 0);
-        for (int i = 0; i < cnt; ++i) {
-          const int j = it.tile(x, i);
-          const uint32_t st = (2 * (base + j) + 1) % NST;
-          if (!count_wait(v_count, base + j + 1, abort_flag) ||
-              (i == 0 && !mbar_wait(&o_free[x], (mine & 1) ^ 1, abort_flag)) ||
-              !mbar_wait(&p_full[x], tiles & 1, abort_flag)) {
-            ok = false;
-            break;
-          }
-          const bool both = i + 1 < cnt && k_ready(i + 1);
-          if (!lock_take(mma_lock, abort_flag)) { ok = false; break; }
-          // P V of this tile and S of the next go out together: the streams'
-          // products then follow one another, and one's softmax runs under the
-          // other's products, instead of both at half speed side by side.
-          ++tiles;
-          tc_fence_after();
-          const uint64_t v_desc =
-              sdesc_sw128(smem_u32(smem + L::kOffKV + st * L::kTile), L::kHalf, 1024);
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            mma_f16_ts(tO, tS + kk * 8, v_desc + kk * (2048 >> 4), kIdescPV,
-                       (i > 0 || kk > 0) ? 1u : 0u);
-          mma_commit(&kv_empty[st]);
-          if (!it.shared(j)) mma_commit(&kv_empty[st]);
-          if (i == cnt - 1) mma_commit(&o_full[x]);
-          if (both) issue_s(i + 1);
-          st_release_cta(mma_lock, 0);
-          if (i + 1 < cnt && !both) {
-            if (!wait_k(i + 1) || !lock_take(mma_lock, abort_flag)) { ok = false; break; }
+        // Step i issues P V of tile i - 1 and S of tile i together: the streams'
+        // products then follow one another, and one's softmax runs under the
+        // other's products, instead of both at half speed side by side. Only
+        // when K of tile i is not there yet, P V goes ahead alone.
+        bool held = false;
+        for (int i = 0; i <= cnt; ++i) {
+          if (i > 0) {
+            const int j = it.tile(x, i - 1);
+            const uint32_t st = (2 * (base + j) + 1) % NST;
+            if (!count_wait(v_count, base + j + 1, abort_flag) ||
+                (i == 1 && !mbar_wait(&o_free[x], (mine & 1) ^ 1, abort_flag)) ||
+                !mbar_wait(&p_full[x], tiles & 1, abort_flag)) {
+              ok = false;
+              break;
+            }
+            ++tiles;
+            const bool both = i < cnt && k_ready(i);
+            if (!lock_take(mma_lock, abort_flag)) { ok = false; break; }
+            held = true;
             tc_fence_after();
-            issue_s(i + 1);
+            const uint64_t v_desc =
+                sdesc_sw128(smem_u32(smem + L::kOffKV + st * L::kTile), L::kHalf, 1024);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+              mma_f16_ts(tO, tS + kk * 8, v_desc + kk * (2048 >> 4), kIdescPV,
+                         (i > 1 || kk > 0) ? 1u : 0u);
+            mma_commit(&kv_empty[st]);
+            if (!it.shared(j)) mma_commit(&kv_empty[st]);
+            if (i == cnt) mma_commit(&o_full[x]);
+            if (!both) {
+              st_release_cta(mma_lock, 0);
+              held = false;
+            }
+          }
+          if (i < cnt) {
+            if (!held) {
+              if (!wait_k(i) || !lock_take(mma_lock, abort_flag)) { ok = false; break; }
+              tc_fence_after();
+            }
+            const int j = it.tile(x, i);
+            const uint32_t st = 2 * (base + j) % NST;
+            const uint64_t k_desc = sdesc_sw128(smem_u32(smem + L::kOffKV + st * L::kTile), 0, 1024);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = ((kk >> 2) * L::kHalf + (kk & 3) * 32) >> 4;
+              mma_f16_ss(tS, q_desc + off, k_desc + off, kIdescQK, kk > 0);
+            }
+            mma_commit(&s_full[x]);
+            // Two arrivals free a slot: one of each stream, or both of its only one.
+            mma_commit(&kv_empty[st]);
+            if (!it.shared(j)) mma_commit(&kv_empty[st]);
+            if (i == cnt - 1) mma_commit(&q_empty[qt]);
             st_release_cta(mma_lock, 0);
+            held = false;
           }
         }
         ++mine;
@@ -839,18 +882,14 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     const uint32_t tS = tmem + x * 128 + lanes, tP = tS, tO = tmem + 256 + x * 128 + lanes;
     const float sl2 = p.scale_log2;
     const int r_tok = r / p.group, r_head = r - r_tok * p.group;
-    Items items;
     RowItem it;
     uint32_t tiles = 0, mine = 0, act1 = 0, alts = 0, ord = 0;
     bool ok = true;
-    for (; ok && items.next(p, tab, it); ++ord) {
+    for (; ok && __all_sync(0xffffffffu, next_item(ord, it)); ++ord) {
       const int cnt = it.count(x);
       if (cnt == 0) {
-        // Looked at, so the list of eight items ago has been given back by both
-        // streams: this arrival cannot be taken for that item's.
-        const bool seen = mbar_wait(&looked[ord % kRowBadBufs], (ord / kRowBadBufs) & 1, abort_flag);
-        if (!__all_sync(0xffffffffu, seen)) break;
-        if (lane == 0) mbar_arrive(&bad_free[ord % kRowBadBufs]);
+        __syncwarp();
+        if (lane == 0) item_done(ord);
         continue;
       }
       const int q_tile = it.alt ? 0 : x;
@@ -871,8 +910,10 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           tmem_ld32(tS + c4 * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c4 * 32]));
         tmem_wait_ld();
         const int k0 = (it.t0 + it.tile(x, i)) * 128;
+        const bool masked = TREE ? k0 + 128 > it.ctx
+                                 : k0 + 127 > it.tok0 + q_tile * p.tile_tokens;
         if constexpr (TREE) {
-          if (k0 + 128 > it.ctx) {
+          if (masked) {
 #pragma unroll
             for (int c4 = 0; c4 < 4; ++c4) {
               const unsigned bits = tree_bits(mask, p.words, it.nodes, k0 + c4 * 32 - it.ctx);
@@ -882,7 +923,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             }
           }
         } else {
-          if (k0 + 127 > it.tok0 + q_tile * p.tile_tokens) {
+          if (masked) {
             const int lim = token - k0;
 #pragma unroll
             for (int c = 0; c < 128; ++c)
@@ -896,14 +937,13 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 #pragma unroll
           for (int u = 0; u < 4; ++u) mx[u] = max3(mx[u], s[c + u], s[c + 4 + u]);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], s[124 + u]);
-        const float mt = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+        for (int u = 0; u < 4; ++u) mx[u] = max2(mx[u], s[124 + u]);
+        const float mt = max2(max3(mx[0], mx[1], mx[2]), mx[3]);
         if (i == 0) {
           m = mt;
           msl = m == -INFINITY ? 0.f : m * sl2;
-        } else if (__any_sync(0xffffffffu, (mt - m) * sl2 > kRowRescale ||
-                                               (m == -INFINITY && mt > -INFINITY))) {
-          const float mn = fmaxf(m, mt);
+        } else if (__any_sync(0xffffffffu, !((mt - m) * sl2 <= kRowRescale))) {
+          const float mn = max2(m, mt);
           const float nsl = mn == -INFINITY ? 0.f : mn * sl2;
           const float alpha = m == -INFINITY ? 0.f : ex2_approx(msl - nsl);
 #pragma unroll 1
@@ -945,9 +985,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       if (it.alt && x == 1) {
         alt_buf[(alts & 1) * 128 + r] = make_float2(m == -INFINITY ? m : msl, l);
         mbar_arrive(&alt_ml[alts & 1]);
-        const bool seen = mbar_wait(&looked[ord % kRowBadBufs], (ord / kRowBadBufs) & 1, abort_flag);
-        if (!__all_sync(0xffffffffu, seen)) break;
-        if (lane == 0) mbar_arrive(&bad_free[ord % kRowBadBufs]);
+        __syncwarp();
+        if (lane == 0) item_done(ord);
         ++alts;
         ++mine;
         continue;
@@ -962,7 +1001,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
               mbar_wait(&o_full[1], act1 & 1, abort_flag);
         if (__all_sync(0xffffffffu, fin)) {
           const float2 o = alt_buf[(alts & 1) * 128 + r];
-          const float mm = fmaxf(ml, o.x);
+          const float mm = max2(ml, o.x);
           // a stream that saw nothing has m = -inf and O = 0
           a0 = ml == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : ex2_approx(ml - mm);
           a1 = o.x == -INFINITY ? 0.f : ex2_approx(o.x - mm);
@@ -971,7 +1010,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         }
         ++alts;
       }
-      fin = fin && mbar_wait(&looked[ord % kRowBadBufs], (ord / kRowBadBufs) & 1, abort_flag);
+      fin = fin && mbar_wait(&looked[ord % kRowItems], (ord / kRowItems) & 1, abort_flag);
       if (!__all_sync(0xffffffffu, fin)) { ok = false; break; }
       ++mine;
       act1 += it.count(1) > 0;
@@ -981,12 +1020,21 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       const int head = it.kh * p.group + r_head;
       // Values that are not finite, of keys this row sees (words of the item's
       // dirty tiles; all zero but for broken inputs).
-      const unsigned* bad = bad_words + (ord % kRowBadBufs) * (kRowMaxDirty * 4);
+      const unsigned* bad = bad_words + (ord % kRowItems) * (kRowMaxDirty * 4);
       const int dirty = first_dirty<TREE>(it);
       const int bad_n = min(max(it.n - dirty, 0), kRowMaxDirty) * 4;
       unsigned any_bad = 0;
       for (int w = 0; w < bad_n; ++w) any_bad |= bad[w];
       float inv = 1.0f;
+      uint8_t* stage = smem + L::kOffOut + warp * 2048;
+      unsigned long long dst = 0;  // where the row goes
+      if (valid)
+        dst = it.part >= 0
+                  ? reinterpret_cast<unsigned long long>(
+                        p.ws_o + (static_cast<long long>(it.part) * 256 + q_tile * 128 + r) * 128)
+                  : reinterpret_cast<unsigned long long>(
+                        static_cast<uint16_t*>(p.out) + row * p.ldo +
+                        static_cast<long long>(head) * D);
       if (it.part < 0) {
         inv = 1.0f / l;
         if constexpr (TREE) {
@@ -1012,39 +1060,59 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 #pragma unroll
           for (int q = 0; q < 32; ++q) o[q] = o[q] * a0 + __uint_as_float(u[q]) * a1;
         }
-        if (any_bad != 0 && valid) {
-          for (int w = 0; w < bad_n; ++w) {
-            for (unsigned b = bad[w]; b != 0; b &= b - 1) {
-              const int k = (it.t0 + dirty) * 128 + w * 32 + __ffs(b) - 1;
-              if (!row_sees<TREE>(it, mask, p.words, token, k)) continue;
-              const uint16_t* vr = value_row<TREE>(p, it, D, k);
-              if (vr == nullptr) continue;
-              vr += c4 * 32;
+        // 64 bytes of a row per lane, turned in shared memory so that four lanes
+        // store each row's piece together (a row per lane would touch 32 lines
+        // with every store).
+        auto put = [&](const uint32_t (&w)[16], int at) {
+          __syncwarp();
 #pragma unroll
-              for (int q = 0; q < 32; ++q)
-                if (nonfinite16<F16>(vr[q])) o[q] += widen16<F16>(vr[q]);
-            }
+          for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ (lane >> 1 & 3)) << 4)) =
+                make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int from = k * 8 + (lane >> 2), c = lane & 3;
+            const unsigned long long to = __shfl_sync(0xffffffffu, dst, from);
+            if (to != 0)
+              *reinterpret_cast<uint4*>(to + at + c * 16) = *reinterpret_cast<const uint4*>(
+                  stage + from * 64 + ((c ^ (from >> 1 & 3)) << 4));
           }
+        };
+        if (it.part >= 0) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t w[16];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) w[q] = __float_as_uint(o[h * 16 + q]);
+            put(w, c4 * 128 + h * 64);
+          }
+        } else {
+          uint32_t w[16];
+#pragma unroll
+          for (int q = 0; q < 16; ++q) w[q] = pack16<F16>(o[2 * q] * inv, o[2 * q + 1] * inv);
+          put(w, c4 * 64);
         }
-        if (valid) {
-          if (it.part >= 0) {
-            float* w = p.ws_o + (static_cast<long long>(it.part) * 256 + q_tile * 128 + r) * 128 +
-                       c4 * 32;
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              reinterpret_cast<float4*>(w)[q] =
-                  make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
-          } else {
-            uint16_t* w = static_cast<uint16_t*>(p.out) + row * p.ldo +
-                          static_cast<long long>(head) * D + c4 * 32;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint4 v;
-              v.x = pack16<F16>(o[8 * q] * inv, o[8 * q + 1] * inv);
-              v.y = pack16<F16>(o[8 * q + 2] * inv, o[8 * q + 3] * inv);
-              v.z = pack16<F16>(o[8 * q + 4] * inv, o[8 * q + 5] * inv);
-              v.w = pack16<F16>(o[8 * q + 6] * inv, o[8 * q + 7] * inv);
-              reinterpret_cast<uint4*>(w)[q] = v;
+      }
+      if (any_bad != 0) {
+        // After the row's own stores: finite + infinity is infinity, and NaN
+        // and opposite infinities come out as they should.
+        __syncwarp();
+        for (int w = 0; valid && w < bad_n; ++w) {
+          for (unsigned b = bad[w]; b != 0; b &= b - 1) {
+            const int k = (it.t0 + dirty) * 128 + w * 32 + __ffs(b) - 1;
+            const uint16_t* vr = value_row<TREE>(p, it, D, k);
+            if (vr == nullptr || !row_sees<TREE>(it, mask, p.words, token, k)) continue;
+#pragma unroll 1
+            for (int d = 0; d < D; ++d) {
+              if (!nonfinite16<F16>(vr[d])) continue;
+              const float add = widen16<F16>(vr[d]);
+              if (it.part >= 0) {
+                reinterpret_cast<float*>(dst)[d] += add;
+              } else {
+                uint16_t* e = reinterpret_cast<uint16_t*>(dst) + d;
+                *e = static_cast<uint16_t>(pack16<F16>(widen16<F16>(*e) + add, 0.f));
+              }
             }
           }
         }
@@ -1056,7 +1124,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       mbar_arrive(&o_free[x]);
       if (it.alt) mbar_arrive(&o_free[1]);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bad_free[ord % kRowBadBufs]);
+      if (lane == 0) item_done(ord);
     }
   }
 
