@@ -14,7 +14,8 @@ int launch_packed(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMa
                   const RowParams& p, int grid, cudaStream_t st) {
   auto kern = row_attn_kernel<D, F16, false>;
   constexpr size_t smem = RowSmem<D>::bytes();
-  if (int rc = row_kernel_ready(kern, smem)) return rc;
+  static std::atomic<uint64_t> ready{0};
+  if (int rc = row_kernel_ready(kern, smem, ready)) return rc;
   kern<<<grid, kRowThreads, smem, st>>>(tq, tk, tv, p);
   KVM_CUDA_TRY(cudaGetLastError());
   return KVM_OK;

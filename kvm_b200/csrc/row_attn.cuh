@@ -49,6 +49,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "ptx.cuh"
@@ -1142,16 +1143,22 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   }
 }
 
-// Before a kernel's launch: its shared memory, and that it was built with the
-// registers its warps hand over to one another (setmaxnreg draws on those of
-// the launch, and a share that is not there is waited for without end).
+// Before a kernel's first launch on a device: its shared memory, and that it
+// was built with the registers its warps hand over to one another (setmaxnreg
+// draws on those of the launch, and a share that is not there is waited for
+// without end). `ready` is the kernel's own flag word, a bit per device.
 template <typename Kern>
-int row_kernel_ready(Kern* kern, size_t smem) {
-  KVM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+int row_kernel_ready(Kern* kern, size_t smem, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  KVM_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (ready.load(std::memory_order_acquire) & bit) return KVM_OK;
   cudaFuncAttributes a;
   KVM_CUDA_TRY(cudaFuncGetAttributes(&a, kern));
   if (a.numRegs * kRowThreads < 256 * kRowSoftmaxRegs + 256 * kRowControlRegs)
     return fail(KVM_ERR_UNSUPPORTED, "attention kernel built with too few registers");
+  KVM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+  ready.fetch_or(bit, std::memory_order_release);
   return KVM_OK;
 }
 

@@ -178,7 +178,8 @@ extern "C" int kvm_sm100_attention_tree_paged(
                               CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   auto kern = row_attn_kernel<128, false, true>;
-  if (int rc = row_kernel_ready(kern, RowSmem<128>::bytes())) return rc;
+  static std::atomic<uint64_t> ready{0};
+  if (int rc = row_kernel_ready(kern, RowSmem<128>::bytes(), ready)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   kern<<<unsigned(ctas), kRowThreads, RowSmem<128>::bytes(), st>>>(tq, tkv, tkv, p);
   KVM_CUDA_TRY(cudaGetLastError());

@@ -18,7 +18,7 @@ import torch
 
 from . import _lib
 from ._lib import call
-from .ops import _check, _rowmajor, _stream
+from .ops import _call_on, _check, _list, _mat, _rowmajor, _stream
 
 
 def kv_strides(layout: str, pages: int, layers: int, block_size: int, width: int):
@@ -136,39 +136,33 @@ class PagedKVCache:
         named by its tree_mask row (int32 [rows, words], bit j % 32 of word
         j / 32 for token j; see tree_mask()). A row that sees nothing is zero.
         Two calls that overlap in time need a workspace each."""
-        _check(q, "q", torch.bfloat16, 2)
-        _check(tree_mask, "tree_mask", torch.int32, 2)
-        for t, n in ((q_offsets, "q_offsets"), (q_positions, "q_positions"),
-                     (block_table, "block_table"), (bt_offsets, "bt_offsets")):
-            self._index(t, n)
-        S, dev = q_positions.numel(), self.pool.device
-        if q_offsets.numel() != S + 1 or bt_offsets.numel() != S + 1:
+        dev = self.pool.get_device()
+        S = _list(q_positions, "q_positions", dev)
+        if _list(q_offsets, "q_offsets", dev) != S + 1 or \
+                _list(bt_offsets, "bt_offsets", dev) != S + 1:
             raise ValueError("q_offsets and bt_offsets must have one more entry than "
                              "q_positions")
-        if q.device != dev or q.shape[1] != heads_q * 128:
-            raise ValueError(f"q must be [rows, {heads_q} * 128] on the pool's device")
-        if tree_mask.shape[0] != q.shape[0] or not tree_mask.is_contiguous() or \
-                tree_mask.device != dev:
-            raise ValueError("tree_mask must be contiguous [rows, words] on the pool's device")
+        _list(block_table, "block_table", dev)
+        if q.dim() != 2 or tree_mask.dim() != 2:
+            raise ValueError("q and tree_mask must be 2-D")
+        rows, words = q.shape[0], tree_mask.shape[1]
+        ldq = _mat(q, "q", torch.bfloat16, rows, heads_q * 128, dev)
+        if _mat(tree_mask, "tree_mask", torch.int32, rows, words, dev) != words and rows > 1:
+            raise ValueError("tree_mask must be contiguous")
         if out is None:
-            out = torch.zeros(q.shape, dtype=q.dtype, device=dev)
-        _check(out, "out", torch.bfloat16, 2)
-        if out.shape != q.shape or out.device != dev:
-            raise ValueError("out must have q's shape and device")
+            out = torch.zeros((rows, heads_q * 128), dtype=q.dtype, device=q.device)
+        ldo = _mat(out, "out", torch.bfloat16, rows, heads_q * 128, dev)
         if workspace is None:
             need = self.tree_workspace(S, heads_q=heads_q, max_q_rows=max_q_rows,
                                        max_keys=max_keys)
-            workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-        elif workspace.device != dev or not workspace.is_contiguous():
+            workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
+        elif workspace.get_device() != dev or not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous on the pool's device")
-        with torch.cuda.device(dev):
-            call("kvm_sm100_attention_tree_paged", q.data_ptr(), _rowmajor(q, "q"),
-                 self.pool.data_ptr(), C.byref(self.layout_struct(layer)), out.data_ptr(),
-                 _rowmajor(out, "out"), q_offsets.data_ptr(), q_positions.data_ptr(),
-                 tree_mask.data_ptr(), tree_mask.shape[1], block_table.data_ptr(),
-                 bt_offsets.data_ptr(), S, q.shape[0], heads_q, max_q_rows, max_keys,
-                 float(scale), workspace.data_ptr(),
-                 workspace.numel() * workspace.element_size(), _stream())
+        _call_on(dev, "kvm_sm100_attention_tree_paged", q.data_ptr(), ldq,
+                 self.pool.data_ptr(), C.byref(self.layout_struct(layer)), out.data_ptr(), ldo,
+                 q_offsets.data_ptr(), q_positions.data_ptr(), tree_mask.data_ptr(), words,
+                 block_table.data_ptr(), bt_offsets.data_ptr(), S, rows, heads_q, max_q_rows,
+                 max_keys, scale, workspace.data_ptr(), workspace.nbytes)
         return out
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
@@ -177,14 +171,12 @@ class PagedKVCache:
         moved within the pool. Sources may repeat; a pair that would race with
         another one (a destination named twice, or also a source) is skipped
         and raises at the next ops.device_status(), as does a bad page id."""
-        for t, n in ((src, "src"), (dst, "dst")):
-            self._index(t, n)
-        if src.shape != dst.shape:
+        dev = self.pool.get_device()
+        n = _list(src, "src", dev)
+        if _list(dst, "dst", dev) != n:
             raise ValueError("src and dst must have the same length")
-        with torch.cuda.device(self.pool.device):
-            call("kvm_sm100_kvcache_copy_pages", self.pool.data_ptr(),
-                 C.byref(self.layout_struct(0)), self.layers, src.data_ptr(), dst.data_ptr(),
-                 src.numel(), _stream())
+        _call_on(dev, "kvm_sm100_kvcache_copy_pages", self.pool.data_ptr(),
+                 C.byref(self.layout_struct(0)), self.layers, src.data_ptr(), dst.data_ptr(), n)
 
     def compact(self, kept: torch.Tensor, kept_offsets: torch.Tensor,
                 q_positions: torch.Tensor, block_table: torch.Tensor,
@@ -194,22 +186,14 @@ class PagedKVCache:
         kept[i] moves to position q_positions[s] + i in every layer. A sequence
         with a bad list or page stays as it is and raises at the next
         ops.device_status()."""
-        for t, n in ((kept, "kept"), (kept_offsets, "kept_offsets"),
-                     (q_positions, "q_positions"), (block_table, "block_table"),
-                     (bt_offsets, "bt_offsets")):
-            self._index(t, n)
-        S = q_positions.numel()
-        if kept_offsets.numel() != S + 1 or bt_offsets.numel() != S + 1:
+        dev = self.pool.get_device()
+        S, n = _list(q_positions, "q_positions", dev), _list(kept, "kept", dev)
+        if _list(kept_offsets, "kept_offsets", dev) != S + 1 or \
+                _list(bt_offsets, "bt_offsets", dev) != S + 1:
             raise ValueError("kept_offsets and bt_offsets must have one more entry than "
                              "q_positions")
-        with torch.cuda.device(self.pool.device):
-            call("kvm_sm100_kvcache_compact", self.pool.data_ptr(),
-                 C.byref(self.layout_struct(0)), self.layers, kept.data_ptr(), kept.numel(),
+        _list(block_table, "block_table", dev)
+        _call_on(dev, "kvm_sm100_kvcache_compact", self.pool.data_ptr(),
+                 C.byref(self.layout_struct(0)), self.layers, kept.data_ptr(), n,
                  kept_offsets.data_ptr(), q_positions.data_ptr(), block_table.data_ptr(),
-                 bt_offsets.data_ptr(), S, _stream())
-
-    def _index(self, t: torch.Tensor, name: str) -> None:
-        """An int32 list on the pool's device."""
-        _check(t, name, torch.int32, 1)
-        if not t.is_contiguous() or t.device != self.pool.device:
-            raise ValueError(f"{name} must be contiguous on the pool's device")
+                 bt_offsets.data_ptr(), S)

@@ -46,6 +46,45 @@ def _rowmajor(t: torch.Tensor, name: str) -> int:
     return t.stride(0)
 
 
+def _mat(t: torch.Tensor, name: str, dtype: torch.dtype, rows: int, cols: int,
+         dev: int) -> int:
+    """Checks a [rows, cols] matrix with contiguous rows on CUDA device `dev`;
+    returns its row stride. (One call per tensor: the small launches of a
+    decode step are bound by the host.)"""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype:
+        raise TypeError(f"{name} must be a {dtype} tensor")
+    if t.get_device() != dev or dev < 0:
+        raise ValueError(f"{name} must be on the CUDA device of the call's other tensors "
+                         "(no CPU path exists)")
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != rows or shape[1] != cols:
+        raise ValueError(f"{name} must be [{rows}, {cols}], got {tuple(shape)}")
+    stride = t.stride()
+    if stride[1] != 1 and cols > 1:
+        raise ValueError(f"{name} must have contiguous rows")
+    return stride[0]
+
+
+def _list(t: torch.Tensor, name: str, dev: int, dtype: torch.dtype = torch.int32) -> int:
+    """Checks a contiguous list on CUDA device `dev`; returns its length."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype:
+        raise TypeError(f"{name} must be a {dtype} tensor")
+    if t.get_device() != dev or dev < 0:
+        raise ValueError(f"{name} must be on the CUDA device of the call's other tensors")
+    if t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous and 1-D")
+    return t.shape[0]
+
+
+def _call_on(dev: int, name: str, *args) -> None:
+    """call(name, *args, stream) with `dev` current and its current stream."""
+    if torch._C._cuda_getDevice() == dev:
+        call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+
+
 # ----------------------------------------------------------------- GEMM ---
 
 def matmul(a: torch.Tensor, b: torch.Tensor, *, b_layout: str = "kn",
@@ -250,25 +289,22 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     offsets[s]:offsets[s+1] (it may be empty). head_dim 64 or 128. Rows that
     belong to no sequence are not written (a new `out` starts as zeros).
     """
-    if not isinstance(q, torch.Tensor) or q.dtype not in _ATTN_DTYPE:
-        raise TypeError("q must be a bf16 or fp16 tensor")
-    for t, n, h in ((q, "q", heads_q), (k, "k", heads_kv), (v, "v", heads_kv)):
-        _check(t, n, q.dtype, 2)
-        if t.shape != (q.shape[0], h * head_dim) or t.device != q.device:
-            raise ValueError(f"{n} must be [{q.shape[0]}, {h} * {head_dim}] on q's device")
-    _check(offsets, "offsets", torch.int32, 1)
-    if offsets.numel() < 1 or not offsets.is_contiguous() or offsets.device != q.device:
-        raise ValueError("offsets must be contiguous [S+1] on q's device")
+    dtype = _ATTN_DTYPE.get(getattr(q, "dtype", None))
+    if dtype is None or q.dim() != 2:
+        raise TypeError("q must be a 2-D bf16 or fp16 tensor")
+    dev, rows, t = q.get_device(), q.shape[0], q.dtype
+    ldq = _mat(q, "q", t, rows, heads_q * head_dim, dev)
+    ldk = _mat(k, "k", t, rows, heads_kv * head_dim, dev)
+    ldv = _mat(v, "v", t, rows, heads_kv * head_dim, dev)
+    n = _list(offsets, "offsets", dev)
+    if n < 1:
+        raise ValueError("offsets must have S+1 entries")
     if out is None:
-        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-    _check(out, "out", q.dtype, 2)
-    if out.shape != q.shape or out.device != q.device:
-        raise ValueError("out must have q's shape and device")
-    with torch.cuda.device(q.device):
-        call("kvm_sm100_attention_packed", q.data_ptr(), _rowmajor(q, "q"), k.data_ptr(),
-             _rowmajor(k, "k"), v.data_ptr(), _rowmajor(v, "v"), out.data_ptr(),
-             _rowmajor(out, "out"), offsets.data_ptr(), offsets.numel() - 1, q.shape[0],
-             heads_q, heads_kv, head_dim, _ATTN_DTYPE[q.dtype], float(scale), _stream())
+        out = torch.zeros((rows, heads_q * head_dim), dtype=t, device=q.device)
+    ldo = _mat(out, "out", t, rows, heads_q * head_dim, dev)
+    _call_on(dev, "kvm_sm100_attention_packed", q.data_ptr(), ldq, k.data_ptr(), ldk,
+             v.data_ptr(), ldv, out.data_ptr(), ldo, offsets.data_ptr(), n - 1, rows, heads_q,
+             heads_kv, head_dim, dtype, scale)
     return out
 
 
@@ -313,19 +349,6 @@ def rope_table(rotary_dim: int, *, base: float = 10000.0, scaling: str = "none",
     return table
 
 
-def _rope_side(x, out, name, rows, heads, head_dim, like):
-    """Checks one of rope's tensors; returns its output."""
-    _check(x, name, like.dtype, 2)
-    if x.shape[0] != rows or x.shape[1] != heads * head_dim or x.device != like.device:
-        raise ValueError(f"{name} must be [{rows}, {heads} * {head_dim}] on the device of q")
-    if out is None:
-        return torch.empty((rows, heads * head_dim), dtype=x.dtype, device=x.device)
-    _check(out, "out of " + name, x.dtype, 2)
-    if out.shape != x.shape or out.device != x.device:
-        raise ValueError(f"out of {name} must have its shape and device")
-    return out
-
-
 def rope(q: torch.Tensor, positions: torch.Tensor, table: _lib.RopeTable, *, heads: int,
          head_dim: int = 128, interleaved: bool = False, backward: bool = False,
          k: torch.Tensor | None = None, heads_kv: int = 0, out: torch.Tensor | None = None,
@@ -341,28 +364,30 @@ def rope(q: torch.Tensor, positions: torch.Tensor, table: _lib.RopeTable, *, hea
     """
     if not isinstance(table, _lib.RopeTable):
         raise TypeError("table must come from rope_table")
-    if not isinstance(q, torch.Tensor) or q.dtype not in _ROPE_DTYPE:
-        raise TypeError("q must be a bf16, fp16 or fp32 tensor")
+    dtype = _ROPE_DTYPE.get(getattr(q, "dtype", None))
+    if dtype is None or q.dim() != 2:
+        raise TypeError("q must be a 2-D bf16, fp16 or fp32 tensor")
     if (k is None) != (heads_kv == 0):
         raise ValueError("k and heads_kv go together")
-    if q.dim() != 2:
-        raise ValueError(f"q must be 2-D, got shape {tuple(q.shape)}")
-    rows = q.shape[0]
-    out = _rope_side(q, out, "q", rows, heads, head_dim, q)
+    dev, rows, t = q.get_device(), q.shape[0], q.dtype
+    ldq = _mat(q, "q", t, rows, heads * head_dim, dev)
+    if out is None:
+        out = torch.empty((rows, heads * head_dim), dtype=t, device=q.device)
+    ldo = _mat(out, "out", t, rows, heads * head_dim, dev)
+    kp = okp = None
+    ldk = ldok = 0
     if k is not None:
-        out_k = _rope_side(k, out_k, "k", rows, heads_kv, head_dim, q)
-    if not positions.is_cuda or positions.dtype not in (torch.int32, torch.int64) or \
-            positions.shape != (rows,) or not positions.is_contiguous() or \
-            positions.device != q.device:
-        raise ValueError("positions must be contiguous int32 or int64 [rows] on q's device")
-    with torch.cuda.device(q.device):
-        call("kvm_sm100_rope", ctypes.byref(table), q.data_ptr(), _rowmajor(q, "q"),
-             out.data_ptr(), _rowmajor(out, "out"), heads,
-             _ptr(k), 0 if k is None else _rowmajor(k, "k"),
-             _ptr(out_k) if k is not None else None,
-             0 if k is None else _rowmajor(out_k, "out_k"), heads_kv, rows, head_dim,
-             int(interleaved), int(backward), _ROPE_DTYPE[q.dtype], positions.data_ptr(),
-             int(positions.dtype == torch.int64), _stream())
+        ldk = _mat(k, "k", t, rows, heads_kv * head_dim, dev)
+        if out_k is None:
+            out_k = torch.empty((rows, heads_kv * head_dim), dtype=t, device=q.device)
+        ldok = _mat(out_k, "out_k", t, rows, heads_kv * head_dim, dev)
+        kp, okp = k.data_ptr(), out_k.data_ptr()
+    wide = positions.dtype is torch.int64
+    if _list(positions, "positions", dev, torch.int64 if wide else torch.int32) != rows:
+        raise ValueError("positions must have one entry per row")
+    _call_on(dev, "kvm_sm100_rope", ctypes.byref(table), q.data_ptr(), ldq, out.data_ptr(), ldo,
+             heads, kp, ldk, okp, ldok, heads_kv, rows, head_dim, interleaved, backward, dtype,
+             positions.data_ptr(), wide)
     return out if k is None else (out, out_k)
 
 

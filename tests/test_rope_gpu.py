@@ -187,7 +187,7 @@ def test_rope_refusals_and_empty(cuda):
             ops.rope(q, pos, table, **kw)
     with pytest.raises(ValueError):
         ops.rope(q, pos[:3], table, heads=2)
-    with pytest.raises(ValueError):
+    with pytest.raises(TypeError):
         ops.rope(q, pos.float(), table, heads=2)
     with pytest.raises(TypeError):
         ops.rope(q.to(torch.float64), pos, table, heads=2)
