@@ -12,8 +12,8 @@ namespace {
 template <int D, bool F16>
 int launch_packed(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                   const RowParams& p, int grid, cudaStream_t st) {
-  auto kern = row_attn_kernel<D, F16, false>;
-  constexpr size_t smem = RowSmem<D>::bytes();
+  auto kern = row_attn_kernel<D, F16, false, false>;
+  constexpr size_t smem = RowSmem<D, false, false>::bytes();
   static std::atomic<uint64_t> ready{0};
   if (int rc = row_kernel_ready(kern, smem, ready)) return rc;
   kern<<<grid, kRowThreads, smem, st>>>(tq, tk, tv, p);

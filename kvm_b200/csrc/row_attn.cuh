@@ -16,7 +16,7 @@
 //                    (shared memory operands), O_x += P_x V_j (P from TMEM:
 //                    shared memory carries Q, K and V reads only, 96 bytes a
 //                    clock at full MMA rate instead of 160)
-//   warp 10          TMA producer of the K and V tiles (one ring for both)
+//   warps 10, 14     TMA producers of the K and of the V tiles, a ring each
 //   warp 11 (1 lane) TMA producer of the Q tiles
 //   warp 12          looks over each V tile that some row must not see whole
 //   warp 13 (1 lane) works out the CTA's next items for the other warps: a ring
@@ -65,30 +65,33 @@ constexpr float kRowRescale = 8.0f;     // log2 units
 constexpr int kRowMaxSeqs = 1024;       // sequences of one call (tables in shared memory)
 constexpr int kRowMaxDirty = 10;        // V tiles of an item that a row sees in part
 constexpr int kRowItems = 4;            // item descriptions in the ring
-constexpr int kRowItemUsers = 13;       // warps that give one back: 0-12
+constexpr int kRowItemUsers = 14;       // warps that give one back: 0-12 and 14
 constexpr int kRowMaxNodes = 1024;
 
-// Shared memory of one CTA for head width D.
-template <int D>
+// Shared memory of one CTA for head width D. ONE: no item has a second Q tile,
+// whose place then goes to the V ring.
+template <int D, bool TREE, bool ONE>
 struct RowSmem {
   static constexpr int kHalves = D / 64;
   static constexpr uint32_t kHalf = 128 * 64 * 2;            // 128 rows x 64 columns
   static constexpr uint32_t kTile = kHalves * kHalf;
-  static constexpr int kStages = D == 128 ? 4 : 8;           // tiles of the K/V ring, K in the even ones
-  static constexpr uint32_t kOffQ = 0;                       // [2]
-  static constexpr uint32_t kOffKV = 2 * kTile;              // [kStages]
-  static constexpr uint32_t kOffTab = kOffKV + kStages * kTile;
-  static constexpr uint32_t kTabBytes = kRowMaxSeqs * 10 + 16;
+  static constexpr int kStagesK = D == 128 ? 2 : 4;
+  static constexpr int kStagesV = kStagesK + (ONE ? 1 : 0);
+  static constexpr uint32_t kOffQ = 0;                       // [2], one with ONE
+  static constexpr uint32_t kOffK = (ONE ? 1 : 2) * kTile;   // [kStagesK]
+  static constexpr uint32_t kOffV = kOffK + kStagesK * kTile;
+  static constexpr uint32_t kOffTab = kOffV + kStagesV * kTile;
+  static constexpr uint32_t kTabBytes = kRowMaxSeqs * (TREE ? 4 : 10) + 16;
   static constexpr uint32_t kOffBad = kOffTab + kTabBytes;
   static constexpr uint32_t kOffItems = kOffBad + kRowItems * kRowMaxDirty * 16;
   static constexpr uint32_t kOffMl = kOffItems + kRowItems * 64;
   static constexpr uint32_t kOffPages = kOffMl + 2 * 128 * 8;
-  static constexpr uint32_t kPageSlots = 128;                // page ids read ahead
-  static constexpr uint32_t kOffOut = kOffPages + kPageSlots * 4;  // [8 warps][32 rows][64 B]
+  static constexpr uint32_t kPageSlots = 128;                // page ids a producer reads ahead
+  static constexpr uint32_t kOffOut = kOffPages + 2 * kPageSlots * 4;  // [8 warps][32 rows][64 B]
   static constexpr uint32_t kOffBar = kOffOut + 8 * 2048;
-  // q_full[2] q_empty[2] kv_full[S] kv_empty[S] s_full[2] p_full[2]
+  // q_full[2] q_empty[2] k_full[] k_empty[] v_full[] v_empty[] s_full[2] p_full[2]
   // o_full[2] o_free[2] alt_ml[2] looked[I] it_full[I] it_empty[I] drain[2]
-  static constexpr int kBars = 2 * kStages + 16 + 3 * kRowItems;
+  static constexpr int kBars = 2 * (kStagesK + kStagesV) + 16 + 3 * kRowItems;
   static constexpr size_t bytes() { return 1024 + kOffBar + kBars * 8 + 16; }
 };
 
@@ -145,14 +148,14 @@ struct RowTables {
   int* total;            // items (prompts) or tiles (trees)
 };
 
-template <int D>
+template <typename L>
 __device__ __forceinline__ RowTables row_tables(uint8_t* smem) {
   RowTables t;
-  uint8_t* p = smem + RowSmem<D>::kOffTab;
+  uint8_t* p = smem + L::kOffTab;
   t.start = reinterpret_cast<int*>(p);
-  t.count = reinterpret_cast<int*>(p + kRowMaxSeqs * 4);
-  t.order = reinterpret_cast<unsigned short*>(p + kRowMaxSeqs * 8);
-  t.total = reinterpret_cast<int*>(p + kRowMaxSeqs * 10);
+  t.count = reinterpret_cast<int*>(p + kRowMaxSeqs * 4);            // prompts
+  t.order = reinterpret_cast<unsigned short*>(p + kRowMaxSeqs * 8);  // prompts
+  t.total = reinterpret_cast<int*>(p + L::kTabBytes - 16);
   return t;
 }
 
@@ -514,23 +517,25 @@ __device__ __forceinline__ float widen16(uint16_t b) {
 
 // -------------------------------------------------------------- kernel ---
 
-template <int D, bool F16, bool TREE>
+template <int D, bool F16, bool TREE, bool ONE>
 __global__ void __launch_bounds__(kRowThreads, 1)
     row_attn_kernel(const __grid_constant__ CUtensorMap tmQ,
                     const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ RowParams p) {
-  using L = RowSmem<D>;
+  using L = RowSmem<D, TREE, ONE>;
   using Items = typename std::conditional<TREE, TreeItems, PromptItems>::type;
-  constexpr int NST = L::kStages;
+  constexpr int NK = L::kStagesK, NV = L::kStagesV;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
   uint64_t* q_full = bars;                      // [2]
   uint64_t* q_empty = q_full + 2;               // [2]
-  uint64_t* kv_full = q_empty + 2;              // [NST]
-  uint64_t* kv_empty = kv_full + NST;           // [NST]
-  uint64_t* s_full = kv_empty + NST;            // [2]
+  uint64_t* k_full = q_empty + 2;               // [NK]
+  uint64_t* k_empty = k_full + NK;              // [NK] 2 arrivals
+  uint64_t* v_full = k_empty + NK;              // [NV]
+  uint64_t* v_empty = v_full + NV;              // [NV] 2 arrivals
+  uint64_t* s_full = v_empty + NV;              // [2]
   uint64_t* p_full = s_full + 2;                // [2] 128 arrivals
   uint64_t* o_full = p_full + 2;                // [2]
   uint64_t* o_free = o_full + 2;                // [2] 128 arrivals
@@ -545,7 +550,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   uint32_t* mma_lock = tmem_slot + 3;
   unsigned* bad_words = reinterpret_cast<unsigned*>(smem + L::kOffBad);
   float2* alt_buf = reinterpret_cast<float2*>(smem + L::kOffMl);   // [2][128]
-  const RowTables tab = row_tables<D>(smem);
+  const RowTables tab = row_tables<L>(smem);
 
   RowItem* ring = reinterpret_cast<RowItem*>(smem + L::kOffItems);
   static_assert(sizeof(RowItem) == 64, "one 64-byte slot each");
@@ -576,9 +581,13 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       mbar_init(&o_free[i], 128);
       mbar_init(&alt_ml[i], 128);
     }
-    for (int i = 0; i < NST; ++i) {
-      mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 2);
+    for (int i = 0; i < NK; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 2);
+    }
+    for (int i = 0; i < NV; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 2);
     }
     for (int i = 0; i < kRowItems; ++i) {
       mbar_init(&looked[i], 1);
@@ -595,7 +604,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     tmem_relinquish();
   }
   if constexpr (TREE) build_tree_tables(p, tab, blockIdx.x == 0);
-  else build_prompt_tables(p, tab, reinterpret_cast<int*>(smem + L::kOffKV));
+  else build_prompt_tables(p, tab, reinterpret_cast<int*>(smem + L::kOffK));
   fence_async_smem();  // the tables' scratch becomes a tile of the ring
   tc_fence_before();
   __syncthreads();
@@ -605,11 +614,17 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 
   if (warp >= 8) {
     reg_give<kRowControlRegs>();
-    if (warp == 10) {
-      // ------------------------------------------------ K/V producer
-      int* page_ids = reinterpret_cast<int*>(smem + L::kOffPages);
+    if (warp == 10 || warp == 14) {
+      // ------------------------------------------------ K and V producers
+      const int kv = warp == 14;
+      const uint32_t N = kv ? NV : NK;
+      uint64_t* full = kv ? v_full : k_full;
+      uint64_t* empty = kv ? v_empty : k_empty;
+      uint8_t* tiles = smem + (kv ? L::kOffV : L::kOffK);
+      const void* map = kv ? &tmV : &tmK;
+      int* page_ids = reinterpret_cast<int*>(smem + L::kOffPages) + kv * L::kPageSlots;
       RowItem it;
-      uint32_t c = 0;  // ring slots filled
+      uint32_t st = 0, phase = 1;  // the ring's next slot
       bool ok = true;
       for (uint32_t ord = 0; ok && __all_sync(0xffffffffu, next_item(ord, it)); ++ord) {
         __syncwarp();
@@ -617,6 +632,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         int have = -1;  // page ids [have, have + kPageSlots) of the sequence are in shared memory
         for (int j = 0; j < it.n && ok; ++j) {
           const int k0 = (it.t0 + j) * 128;
+          uint8_t* dst = tiles + st * L::kTile;
           if constexpr (TREE) {
             const int k1 = min(k0 + 128, it.keys);
             const int pg0 = k0 / p.block_size, pg1 = (k1 - 1) / p.block_size;
@@ -637,47 +653,39 @@ __global__ void __launch_bounds__(kRowThreads, 1)
               }
               __syncwarp();
             }
+            // lane i issues the boxes of the tile's i-th page
             const int segs = (k1 - k0 + p.box_rows - 1) / p.box_rows;
             const int tok = k0 + lane * p.box_rows;
             const int page = lane < segs ? page_ids[tok / p.block_size - have] : -1;
             const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
-            const uint32_t bytes = boxes * p.box_rows * (D * 2u);
-#pragma unroll
-            for (int kv = 0; kv < 2; ++kv) {
-              const uint32_t st = c % NST;
-              bool got = true;
-              if (lane == 0) {
-                got = mbar_wait(&kv_empty[st], ((c / NST) & 1) ^ 1, abort_flag);
-                if (got) mbar_arrive_expect_tx(&kv_full[st], bytes);
-              }
-              ok = __shfl_sync(0xffffffffu, got, 0);
-              if (!ok) break;
-              if (page >= 0) {
-                const int row = static_cast<int>(page * p.page_rows + p.layer * p.layer_rows +
-                                                 kv * p.kv_rows + tok % p.block_size);
-                uint8_t* dst = smem + L::kOffKV + st * L::kTile + lane * p.box_rows * 128u;
-#pragma unroll
-                for (int h = 0; h < L::kHalves; ++h)
-                  tma_load_2d(dst + h * L::kHalf, &tmK, &kv_full[st], it.kh * D + h * 64, row);
-              }
-              ++c;
+            bool got = true;
+            if (lane == 0) {
+              got = mbar_wait(&empty[st], phase, abort_flag);
+              if (got) mbar_arrive_expect_tx(&full[st], boxes * p.box_rows * (D * 2u));
             }
-          } else if (lane == 0) {
-#pragma unroll
-            for (int kv = 0; kv < 2; ++kv) {
-              const uint32_t st = c % NST;
-              if (!mbar_wait(&kv_empty[st], ((c / NST) & 1) ^ 1, abort_flag)) {
-                ok = false;
-                break;
-              }
-              mbar_arrive_expect_tx(&kv_full[st], L::kTile);
-              uint8_t* dst = smem + L::kOffKV + st * L::kTile;
+            ok = __shfl_sync(0xffffffffu, got, 0);
+            if (!ok) break;
+            if (page >= 0) {
+              const int row = static_cast<int>(page * p.page_rows + p.layer * p.layer_rows +
+                                               kv * p.kv_rows + tok % p.block_size);
+              dst += lane * p.box_rows * 128u;
 #pragma unroll
               for (int h = 0; h < L::kHalves; ++h)
-                tma_load_2d(dst + h * L::kHalf, kv ? &tmV : &tmK, &kv_full[st],
-                            it.kh * D + h * 64, it.key0 + k0);
-              ++c;
+                tma_load_2d(dst + h * L::kHalf, map, &full[st], it.kh * D + h * 64, row);
             }
+          } else if (lane == 0) {
+            if (!mbar_wait(&empty[st], phase, abort_flag)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive_expect_tx(&full[st], L::kTile);
+#pragma unroll
+            for (int h = 0; h < L::kHalves; ++h)
+              tma_load_2d(dst + h * L::kHalf, map, &full[st], it.kh * D + h * 64, it.key0 + k0);
+          }
+          if (++st == N) {
+            st = 0;
+            phase ^= 1;
           }
         }
         __syncwarp();
@@ -712,11 +720,11 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         const int dirty = first_dirty<TREE>(it);
         unsigned* bad = bad_words + (ord % kRowItems) * (kRowMaxDirty * 4);
         for (int j = 0; j < it.n; ++j, ++c) {
-          const uint32_t slot = 2 * c + 1, st = slot % NST;
-          const bool in = mbar_wait(&kv_full[st], (slot / NST) & 1, abort_flag);
+          const uint32_t st = c % NV;
+          const bool in = mbar_wait(&v_full[st], (c / NV) & 1, abort_flag);
           if (!__all_sync(0xffffffffu, in)) { ok = false; break; }
           if (j >= dirty) {
-            uint8_t* tile = smem + L::kOffKV + st * L::kTile;
+            uint8_t* tile = smem + L::kOffV + st * L::kTile;
 #pragma unroll 1
             for (int q = 0; q < 4; ++q) {
               const int r = q * 32 + lane;
@@ -800,14 +808,14 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         if (x == 1 && !it.alt) mbar_arrive(&q_empty[0]);
         const uint64_t q_desc = sdesc_sw128(smem_u32(smem + L::kOffQ + qt * L::kTile), 0, 1024);
         auto k_ready = [&](int i) {
-          const uint32_t slot = 2 * (base + it.tile(x, i));
-          return mbar_test(&kv_full[slot % NST], (slot / NST) & 1);
+          const uint32_t g = base + it.tile(x, i);
+          return mbar_test(&k_full[g % NK], (g / NK) & 1);
         };
         // K of the stream's i-th tile (and its Q tile) are in shared memory.
         auto wait_k = [&](int i) {
-          const uint32_t slot = 2 * (base + it.tile(x, i));
+          const uint32_t g = base + it.tile(x, i);
           return (i > 0 || !qt || mbar_wait(&q_full[1], ord1 & 1, abort_flag)) &&
-                 mbar_wait(&kv_full[slot % NST], (slot / NST) & 1, abort_flag);
+                 mbar_wait(&k_full[g % NK], (g / NK) & 1, abort_flag);
         };
         if (cnt == 0) continue;
         // Step i issues P V of tile i - 1 and S of tile i together: the streams'
@@ -818,7 +826,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         for (int i = 0; i <= cnt; ++i) {
           if (i > 0) {
             const int j = it.tile(x, i - 1);
-            const uint32_t st = (2 * (base + j) + 1) % NST;
+            const uint32_t st = (base + j) % NV;
             if (!count_wait(v_count, base + j + 1, abort_flag) ||
                 (i == 1 && !mbar_wait(&o_free[x], (mine & 1) ^ 1, abort_flag)) ||
                 !mbar_wait(&p_full[x], tiles & 1, abort_flag)) {
@@ -831,13 +839,13 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             held = true;
             tc_fence_after();
             const uint64_t v_desc =
-                sdesc_sw128(smem_u32(smem + L::kOffKV + st * L::kTile), L::kHalf, 1024);
+                sdesc_sw128(smem_u32(smem + L::kOffV + st * L::kTile), L::kHalf, 1024);
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk)
               mma_f16_ts(tO, tS + kk * 8, v_desc + kk * (2048 >> 4), kIdescPV,
                          (i > 1 || kk > 0) ? 1u : 0u);
-            mma_commit(&kv_empty[st]);
-            if (!it.shared(j)) mma_commit(&kv_empty[st]);
+            mma_commit(&v_empty[st]);
+            if (!it.shared(j)) mma_commit(&v_empty[st]);
             if (i == cnt) mma_commit(&o_full[x]);
             if (!both) {
               st_release_cta(mma_lock, 0);
@@ -850,8 +858,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
               tc_fence_after();
             }
             const int j = it.tile(x, i);
-            const uint32_t st = 2 * (base + j) % NST;
-            const uint64_t k_desc = sdesc_sw128(smem_u32(smem + L::kOffKV + st * L::kTile), 0, 1024);
+            const uint32_t st = (base + j) % NK;
+            const uint64_t k_desc = sdesc_sw128(smem_u32(smem + L::kOffK + st * L::kTile), 0, 1024);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
               const uint32_t off = ((kk >> 2) * L::kHalf + (kk & 3) * 32) >> 4;
@@ -859,8 +867,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             }
             mma_commit(&s_full[x]);
             // Two arrivals free a slot: one of each stream, or both of its only one.
-            mma_commit(&kv_empty[st]);
-            if (!it.shared(j)) mma_commit(&kv_empty[st]);
+            mma_commit(&k_empty[st]);
+            if (!it.shared(j)) mma_commit(&k_empty[st]);
             if (i == cnt - 1) mma_commit(&q_empty[qt]);
             st_release_cta(mma_lock, 0);
             held = false;

@@ -81,6 +81,18 @@ __global__ void __launch_bounds__(kJoinThreads)
   }
 }
 
+template <bool ONE>
+int launch_tree(const CUtensorMap& tq, const CUtensorMap& tkv, const RowParams& p, int ctas,
+                cudaStream_t st) {
+  auto kern = row_attn_kernel<128, false, true, ONE>;
+  constexpr size_t smem = RowSmem<128, true, ONE>::bytes();
+  static std::atomic<uint64_t> ready{0};
+  if (int rc = row_kernel_ready(kern, smem, ready)) return rc;
+  kern<<<ctas, kRowThreads, smem, st>>>(tq, tkv, tkv, p);
+  KVM_CUDA_TRY(cudaGetLastError());
+  return KVM_OK;
+}
+
 // CTAs of a call: one per four key tiles of the largest it may be.
 int64_t tree_ctas(int64_t S, int HKV, int group, int max_q_rows, int max_keys) {
   const int64_t per = 2 * (128 / group);
@@ -177,12 +189,11 @@ extern "C" int kvm_sm100_attention_tree_paged(
                               p.box_rows, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                               CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
-  auto kern = row_attn_kernel<128, false, true>;
-  static std::atomic<uint64_t> ready{0};
-  if (int rc = row_kernel_ready(kern, RowSmem<128>::bytes(), ready)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  kern<<<unsigned(ctas), kRowThreads, RowSmem<128>::bytes(), st>>>(tq, tkv, tkv, p);
-  KVM_CUDA_TRY(cudaGetLastError());
+  // Trees that fit one Q tile leave the second one's place to the V ring.
+  const int rc = max_q_rows <= p.tile_tokens ? launch_tree<true>(tq, tkv, p, int(ctas), st)
+                                             : launch_tree<false>(tq, tkv, p, int(ctas), st);
+  if (rc != KVM_OK) return rc;
   if (ctas > 1) {
     const int most = int64_t(max_q_rows) < per ? max_q_rows : int(per);
     const int last_row = most <= p.tile_tokens ? most * group : 128 + (most - p.tile_tokens) * group;
