@@ -39,6 +39,8 @@ __global__ void __launch_bounds__(kCopyThreads)
     copy_pages_kernel(uint4* __restrict__ pool, const __grid_constant__ PageRuns r,
                       const int* __restrict__ src, const int* __restrict__ dst, int n,
                       int num_pages, int chunks, long long steps, int* status) {
+  pdl_wait();
+  pdl_trigger();
   const long long per = (steps + gridDim.x - 1) / gridDim.x;
   const long long begin = blockIdx.x * per, end = min(begin + per, steps);
   int pair = -1;
@@ -92,6 +94,8 @@ __global__ void __launch_bounds__(kCompactThreads)
                    const int* __restrict__ kept_off, const int* __restrict__ q_pos,
                    const int* __restrict__ bt, const int* __restrict__ bt_off, int* status) {
   __shared__ long long from[kCompactBatch], to[kCompactBatch];
+  pdl_wait();
+  pdl_trigger();
   const int unit = blockIdx.x;
   const int kv = unit & 1, layer = L.layer + (unit >> 1) % layers, s = (unit >> 1) / layers;
   const int k0 = kept_off[s], m = kept_off[s + 1] - k0;
@@ -187,9 +191,9 @@ extern "C" int kvm_sm100_kvcache_copy_pages(void* cache, const kvm_kv_layout* L,
   const long long steps = static_cast<long long>(n) * chunks;
   const long long most = dev->sm_count * 8ll;
   const int grid = static_cast<int>(steps < most ? steps : most);
-  copy_pages_kernel<<<grid, kCopyThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-      base, r, src, dst, n, L->num_pages, chunks, steps, dev->status);
-  KVM_CUDA_TRY(cudaGetLastError());
+  KVM_CUDA_TRY(launch_ex(true, copy_pages_kernel, dim3(grid), dim3(kCopyThreads), 0,
+                         static_cast<cudaStream_t>(stream), base, r, src, dst, n, L->num_pages,
+                         chunks, steps, dev->status));
   return KVM_OK;
 }
 
@@ -211,10 +215,9 @@ extern "C" int kvm_sm100_kvcache_compact(void* cache, const kvm_kv_layout* L, in
     return fail(KVM_ERR_INVALID_ARG, "kvcache_compact: too many sequences and layers");
   const DeviceInfo* dev = device_info();
   if (!dev) return KVM_ERR_CUDA;
-  compact_kernel<<<static_cast<unsigned>(blocks), kCompactThreads, 0,
-                   static_cast<cudaStream_t>(stream)>>>(
-      static_cast<uint4*>(cache), *L, layers, kept, n_kept, kept_offsets, q_positions, block_table,
-      bt_offsets, dev->status);
-  KVM_CUDA_TRY(cudaGetLastError());
+  KVM_CUDA_TRY(launch_ex(true, compact_kernel, dim3(static_cast<unsigned>(blocks)),
+                         dim3(kCompactThreads), 0, static_cast<cudaStream_t>(stream),
+                         static_cast<uint4*>(cache), *L, layers, kept, n_kept, kept_offsets,
+                         q_positions, block_table, bt_offsets, dev->status));
   return KVM_OK;
 }

@@ -16,8 +16,7 @@ int launch_packed(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMa
   constexpr size_t smem = RowSmem<D, false, false>::bytes();
   static std::atomic<uint64_t> ready{0};
   if (int rc = row_kernel_ready(kern, smem, ready)) return rc;
-  kern<<<grid, kRowThreads, smem, st>>>(tq, tk, tv, p);
-  KVM_CUDA_TRY(cudaGetLastError());
+  KVM_CUDA_TRY(launch_ex(true, kern, dim3(grid), dim3(kRowThreads), smem, st, tq, tk, tv, p));
   return KVM_OK;
 }
 

@@ -84,6 +84,8 @@ __global__ void __launch_bounds__(kRopeThreads)
   const int half = p.rot / 2;
   const int col = rotates ? unit * V : p.rot + (unit - p.rot_units) * V;
 
+  pdl_wait();
+  pdl_trigger();
   W a[kRopeUnroll], b[kRopeUnroll];
 #pragma unroll
   for (int u = 0; u < kRopeUnroll; ++u) {
@@ -168,11 +170,8 @@ cudaError_t rope_launch(RopeParams p, const kvm_rope_table& t, int rows, int sms
   p.heads_per_block = p.slots * it;
   const dim3 grid(rows, (total + p.heads_per_block - 1) / p.heads_per_block);
   const int threads = (p.slots * p.units + 31) / 32 * 32;
-  if (vec)
-    rope_rows_kernel<T, V16, INTER><<<grid, threads, 0, st>>>(p, t);
-  else
-    rope_rows_kernel<T, V1, INTER><<<grid, threads, 0, st>>>(p, t);
-  return cudaGetLastError();
+  return launch_ex(true, vec ? rope_rows_kernel<T, V16, INTER> : rope_rows_kernel<T, V1, INTER>,
+                   grid, dim3(threads), 0, st, p, t);
 }
 
 }  // namespace

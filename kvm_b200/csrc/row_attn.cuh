@@ -111,6 +111,7 @@ struct RowParams {
   const int* q_pos;      // [S] cached tokens before the tree
   const unsigned* mask;  // [rows, words]
   int words, max_nodes, max_keys;
+  int whole;             // items are not cut
   const int* bt;
   const int* bt_off;
   int block_size, box_rows, num_pages, layer;
@@ -142,7 +143,7 @@ struct RowItem {
 
 // Tables in shared memory, built once per CTA from the offsets on the device.
 struct RowTables {
-  int* start;            // prompts: first item of rank r's block; trees: first tile of s
+  int* start;            // prompts: first item of rank r's block; trees: first tile (item) of s
   int* count;            // prompts: items of the sequence of rank r
   unsigned short* order; // prompts: sequence of rank r
   int* total;            // items (prompts) or tiles (trees)
@@ -248,8 +249,8 @@ struct PromptItems {
 // The key tiles of all (sequence, query tile pair, kv head) in a row, in that
 // order, are cut into one stretch of equal length per CTA: every CTA streams
 // the same number of K/V tiles whatever the contexts. A stretch that begins
-// or ends inside an item leaves a partial result; the combine kernel joins
-// them.
+// or ends inside an item leaves a partial result; the joining kernel joins
+// them. A few short items (`whole`) are dealt out uncut instead, one to a CTA.
 __device__ __forceinline__ int tree_pairs(const RowParams& p, int nodes) {
   return (nodes + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
 }
@@ -276,7 +277,7 @@ __device__ __forceinline__ void build_tree_tables(const RowParams& p, RowTables 
       if (s < p.S) {
         int nodes, ctx;
         const int tiles = tree_tiles(p, s, nodes, ctx, report);
-        n = tiles * tree_pairs(p, nodes) * p.HKV;
+        n = (p.whole ? tiles > 0 : tiles) * tree_pairs(p, nodes) * p.HKV;
       }
       int sum = n;
 #pragma unroll
@@ -301,7 +302,7 @@ struct TreeItems {
   int pos = -1, end = 0, first = 1;
   __device__ __forceinline__ bool next(const RowParams& p, const RowTables& t, RowItem& it) {
     if (pos < 0) {
-      const int total = *t.total, share = tree_share(total, gridDim.x);
+      const int total = *t.total, share = p.whole ? 1 : tree_share(total, gridDim.x);
       const long long b = static_cast<long long>(blockIdx.x) * share;
       pos = b < total ? static_cast<int>(b) : total;
       end = min(pos + share, total);
@@ -315,14 +316,14 @@ struct TreeItems {
     it.s = lo;
     const int tiles = tree_tiles(p, lo, it.nodes, it.ctx, false);
     const int at = pos - t.start[lo];
-    const int item = at / tiles;
+    const int item = p.whole ? at : at / tiles;
     it.kh = item % p.HKV;
     it.tok0 = item / p.HKV * 2 * p.tile_tokens;
     it.key0 = 0;
     it.row0 = p.q_off[lo] + it.tok0;
     it.keys = it.ctx + it.nodes;
-    it.t0 = at - item * tiles;
-    it.n = min(tiles - it.t0, end - pos);
+    it.t0 = p.whole ? 0 : at - item * tiles;
+    it.n = p.whole ? tiles : min(tiles - it.t0, end - pos);
     const int left = it.nodes - it.tok0;
     it.ntok0 = min(left, p.tile_tokens);
     it.ntok1 = max(0, min(left - p.tile_tokens, p.tile_tokens));
@@ -331,7 +332,7 @@ struct TreeItems {
     it.alt = it.ntok1 == 0 && it.n > 1;
     it.part = it.n == tiles ? -1 : 2 * int(blockIdx.x) + (first ? 0 : 1);
     first = 0;
-    pos += it.n;
+    pos = p.whole ? end : pos + it.n;
     return true;
   }
 };
@@ -603,6 +604,10 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  // All before this may overlap the kernel ahead in the stream; what follows
+  // reads what it may have written.
+  pdl_wait();
+  pdl_trigger();
   if constexpr (TREE) build_tree_tables(p, tab, blockIdx.x == 0);
   else build_prompt_tables(p, tab, reinterpret_cast<int*>(smem + L::kOffK));
   fence_async_smem();  // the tables' scratch becomes a tile of the ring

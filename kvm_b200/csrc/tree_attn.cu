@@ -28,6 +28,11 @@ __global__ void __launch_bounds__(kJoinThreads)
   const int total = total_s, share = tree_share(total, ctas), c = blockIdx.x;
   const long long begin = static_cast<long long>(c) * share;
   const long long end = begin + share;
+  // The partial results are the kernel's before this one. (The offsets are not:
+  // it has waited for their writers before letting this one start.) No block
+  // may leave before: this kernel would then end before that one does.
+  pdl_wait();
+  pdl_trigger();
   if (end >= total) return;          // nothing goes on after the last stretch
   int lo = 0, hi = p.S - 1;
   while (lo < hi) {
@@ -43,7 +48,6 @@ __global__ void __launch_bounds__(kJoinThreads)
   const int last = static_cast<int>((i1 - 1) / share);
   const int slot0 = 2 * c + (i0 == begin ? 0 : 1);
   const int lane = threadIdx.x % 32;
-  pdl_wait();                        // the partial results are the kernel's before this one
   for (int r = blockIdx.y * kJoinRows + threadIdx.x / 32; r < (blockIdx.y + 1) * kJoinRows;
        r += kJoinThreads / 32) {
     const int q_tile = r >> 7, in_tile = r & 127;
@@ -88,17 +92,25 @@ int launch_tree(const CUtensorMap& tq, const CUtensorMap& tkv, const RowParams& 
   constexpr size_t smem = RowSmem<128, true, ONE>::bytes();
   static std::atomic<uint64_t> ready{0};
   if (int rc = row_kernel_ready(kern, smem, ready)) return rc;
-  kern<<<ctas, kRowThreads, smem, st>>>(tq, tkv, tkv, p);
-  KVM_CUDA_TRY(cudaGetLastError());
+  KVM_CUDA_TRY(launch_ex(true, kern, dim3(ctas), dim3(kRowThreads), smem, st, tq, tkv, tkv, p));
   return KVM_OK;
 }
 
-// CTAs of a call: one per four key tiles of the largest it may be.
-int64_t tree_ctas(int64_t S, int HKV, int group, int max_q_rows, int max_keys) {
+// How a call is cut up, from its bounds alone.
+struct TreeCut {
+  int64_t ctas;
+  bool whole;
+};
+TreeCut tree_cut(int64_t S, int HKV, int group, int max_q_rows, int max_keys) {
   const int64_t per = 2 * (128 / group);
-  const int64_t tiles = S * HKV * ((max_q_rows + per - 1) / per) * ((int64_t(max_keys) + 127) / 128);
-  const int64_t ctas = (tiles + 3) / 4;
-  return ctas < kTreeMaxCtas ? ctas : kTreeMaxCtas;
+  const int64_t items = S * HKV * ((max_q_rows + per - 1) / per);
+  const int64_t tiles = (int64_t(max_keys) + 127) / 128;
+  // Items that fit the CTAs one each, of at most eight key tiles, stay whole:
+  // cutting them saves at most half of their few microseconds and costs the
+  // joining launch.
+  if (items <= kTreeMaxCtas && tiles <= 8) return {items, true};
+  const int64_t ctas = (items * tiles + 3) / 4;  // four key tiles each, at least
+  return {ctas < kTreeMaxCtas ? ctas : kTreeMaxCtas, false};
 }
 
 }  // namespace
@@ -111,7 +123,8 @@ extern "C" int64_t kvm_sm100_attention_tree_workspace(int S, int HQ, int HKV, in
   if (S <= 0 || HQ <= 0 || HKV <= 0 || HQ % HKV || HQ / HKV > 128 || max_q_rows <= 0 ||
       max_keys <= 0)
     return 0;
-  return tree_ctas(S, HKV, HQ / HKV, max_q_rows, max_keys) * 2 * 256 * (128 + 2) * 4;
+  const TreeCut cut = tree_cut(S, HKV, HQ / HKV, max_q_rows, max_keys);
+  return cut.whole ? 0 : cut.ctas * 2 * 256 * (128 + 2) * 4;
 }
 
 extern "C" int kvm_sm100_attention_tree_paged(
@@ -156,9 +169,10 @@ extern "C" int kvm_sm100_attention_tree_paged(
                             int64_t(L->layer) * (L->layer_stride / L->token_stride) + L->kv_stride / L->token_stride + bs;
   if (pool_rows >= (1ll << 31))
     return fail(KVM_ERR_UNSUPPORTED, "attention_tree: pool too large for 32-bit rows");
-  const int64_t ctas = tree_ctas(S, HKV, group, max_q_rows, max_keys);
+  const TreeCut cut = tree_cut(S, HKV, group, max_q_rows, max_keys);
+  const int64_t ctas = cut.ctas;
   const int64_t need = kvm_sm100_attention_tree_workspace(S, HQ, HKV, max_q_rows, max_keys);
-  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(KVM_ERR_INVALID_ARG, "attention_tree: workspace too small");
   const DeviceInfo* dev = device_info();
   if (!dev) return KVM_ERR_CUDA;
@@ -170,7 +184,7 @@ extern "C" int kvm_sm100_attention_tree_paged(
   p.out = out; p.ldo = ldo; p.q_off = q_offsets; p.status = dev->status;
   p.v = cache; p.ldv = L->token_stride;
   p.q_pos = q_positions; p.mask = mask; p.words = mask_words;
-  p.max_nodes = max_q_rows; p.max_keys = max_keys;
+  p.max_nodes = max_q_rows; p.max_keys = max_keys; p.whole = cut.whole;
   p.bt = block_table; p.bt_off = bt_offsets;
   p.block_size = bs; p.box_rows = bs < 128 ? bs : 128;
   p.num_pages = L->num_pages; p.layer = L->layer;
@@ -178,7 +192,7 @@ extern "C" int kvm_sm100_attention_tree_paged(
   p.layer_rows = L->layer_stride / L->token_stride;
   p.kv_rows = L->kv_stride / L->token_stride;
   p.ws_o = static_cast<float*>(workspace);
-  p.ws_ml = p.ws_o + ctas * 2 * 256 * 128;
+  p.ws_ml = need > 0 ? p.ws_o + ctas * 2 * 256 * 128 : nullptr;
   CUtensorMap tq, tkv;
   if (int rc = encode_tmap_3d(&tq, q, {128, uint64_t(HQ), uint64_t(rows)},
                               {256, uint64_t(ldq) * 2},
@@ -194,12 +208,11 @@ extern "C" int kvm_sm100_attention_tree_paged(
   const int rc = max_q_rows <= p.tile_tokens ? launch_tree<true>(tq, tkv, p, int(ctas), st)
                                              : launch_tree<false>(tq, tkv, p, int(ctas), st);
   if (rc != KVM_OK) return rc;
-  if (ctas > 1) {
+  if (!cut.whole && ctas > 1) {
     const int most = int64_t(max_q_rows) < per ? max_q_rows : int(per);
     const int last_row = most <= p.tile_tokens ? most * group : 128 + (most - p.tile_tokens) * group;
     const dim3 grid(unsigned(ctas - 1), (last_row + kJoinRows - 1) / kJoinRows);
     KVM_CUDA_TRY(launch_ex(true, tree_join_kernel, grid, dim3(kJoinThreads), 0, st, p, int(ctas)));
-    KVM_CUDA_TRY(cudaGetLastError());
   }
   return KVM_OK;
 }

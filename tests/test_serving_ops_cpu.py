@@ -180,11 +180,11 @@ def test_attention_tree_refuses_without_a_gpu():
     assert rc(a12=1025) == UNS and rc(a15=0) == INV and rc(a15=1025, a9=64) == INV
     assert rc(a15=33) == INV and rc(a16=0) == INV and rc(a17=float("nan")) == INV
     assert rc(a0=None) == INV and rc(a4=P + 4) == INV and rc(a8=None) == INV and rc(a1=1000) == INV
-    assert rc(a18=None) == INV and rc(a19=100) == INV
+    assert rc(a18=None, a16=2000) == INV and rc(a19=100, a16=2000) == INV
     assert rc(layout=dict(num_pages=1 << 30, page_stride=1 << 20)) == UNS
     assert rc(a12=0) == _lib.KVM_OK and rc(a13=0) == _lib.KVM_OK
     ws = _lib.lib().kvm_sm100_attention_tree_workspace
     assert ws(0, 8, 2, 5, 100) == 0 and ws(2, 7, 2, 5, 100) == 0 and ws(2, 8, 2, 0, 100) == 0
-    # one stretch for the two sequences' four one-tile items
-    assert ws(2, 8, 2, 5, 100) == 2 * 256 * 130 * 4
+    assert ws(2, 8, 2, 5, 1024) == 0      # four short items are not cut
+    assert ws(2, 8, 2, 5, 1025) == 9 * 2 * 256 * 130 * 4    # 36 key tiles, four to a CTA
     assert ws(64, 64, 8, 16, 5000) == 148 * 2 * 256 * 130 * 4

@@ -185,7 +185,7 @@ def test_tree_scale_out_workspace_and_rows_left_alone(cuda):
     check(wide[:rows, :1024], ref, mag * (1 + 4 * 2.0 ** -5), 1508)
     assert bool((wide[rows:] == 5).all()) and bool((wide[:, 1024:] == 5).all())
     with pytest.raises(KvmError):
-        c.run(workspace=ws[:16])
+        c.run(workspace=ws[:16], max_keys=2000)
 
 
 def test_tree_out_of_bounds_sequences_are_reported(cuda):
