@@ -32,7 +32,11 @@ namespace kvm {
 namespace {
 
 constexpr int kRopeThreads = 256;
-constexpr int kRopeUnroll = 4;
+// Units in flight per thread: 64 bytes of loads in either layout. (Four split
+// units take 106 registers; at two blocks an SM 8192 rows of 72 heads took 101
+// us instead of 58.)
+template <bool INTER>
+constexpr int kRopeUnroll = INTER ? 4 : 2;
 
 struct RopeSide {
   const void* x;
@@ -71,7 +75,7 @@ struct alignas(sizeof(T) * V == 16 ? 16 : alignof(T)) Vec {
 // V: elements of a vector. Split layout: a rotating unit is the vectors at j
 // and j + rot/2; interleaved: one vector holding V/2 pairs.
 template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(kRopeThreads)
+__global__ void __launch_bounds__(kRopeThreads, 4)
     rope_rows_kernel(const __grid_constant__ RopeParams p,
                      const __grid_constant__ kvm_rope_table t) {
   __shared__ float2 cs[KVM_ROPE_MAX_PAIRS];
@@ -86,9 +90,10 @@ __global__ void __launch_bounds__(kRopeThreads)
 
   pdl_wait();
   pdl_trigger();
-  W a[kRopeUnroll], b[kRopeUnroll];
+  constexpr int U = kRopeUnroll<INTER>;
+  W a[U], b[U];
 #pragma unroll
-  for (int u = 0; u < kRopeUnroll; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int h = h0 + slot + u * p.slots;
     if (slot < p.slots && h < heads) {
       const bool is_q = h < p.q.heads;
@@ -100,6 +105,7 @@ __global__ void __launch_bounds__(kRopeThreads)
     }
   }
 
+  constexpr int NP = INTER ? V / 2 : V;  // pairs of a unit
   const long long pos = p.pos64 ? static_cast<const long long*>(p.positions)[row]
                                 : static_cast<const int*>(p.positions)[row];
   for (int i = threadIdx.x; i < t.pairs; i += blockDim.x) {
@@ -108,18 +114,18 @@ __global__ void __launch_bounds__(kRopeThreads)
     const float half_turns = static_cast<float>(static_cast<int>(turn >> 32)) * 0x1p-31f;
     float sn, cn;
     sincospif(half_turns, &sn, &cn);
-    cs[i] = make_float2(cn * t.magnitude, sn * t.magnitude * p.sign);
+    // a unit's pairs rot_units apart: the units of a warp read without conflicts
+    cs[i % NP * p.rot_units + i / NP] = make_float2(cn * t.magnitude, sn * t.magnitude * p.sign);
   }
   __syncthreads();
 
-  constexpr int NP = INTER ? V / 2 : V;  // pairs of a unit
   float2 w[NP];
   if (rotates) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) w[i] = cs[unit * NP + i];
+    for (int i = 0; i < NP; ++i) w[i] = cs[i * p.rot_units + unit];
   }
 #pragma unroll
-  for (int u = 0; u < kRopeUnroll; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int h = h0 + slot + u * p.slots;
     if (slot < p.slots && h < heads) {
       const bool is_q = h < p.q.heads;
@@ -158,15 +164,28 @@ cudaError_t rope_launch(RopeParams p, const kvm_rope_table& t, int rows, int sms
   const int v = vec ? V16 : V1;
   p.rot_units = (INTER ? p.rot : p.rot / 2) / v;
   p.units = p.rot_units + (p.head_dim - p.rot) / v;
-  p.slots = kRopeThreads / p.units;
   const int total = p.q.heads + p.k.heads;
-  if (p.slots > total) p.slots = total;
+  const int most = kRopeThreads / p.units < total ? kRopeThreads / p.units : total;
   // One pass of the slots per block while that leaves SMs idle, else up to
-  // kRopeUnroll, which spreads a row's sines over more of its heads.
-  const int passes = (total + p.slots - 1) / p.slots;
-  const int it = static_cast<long long>(rows) * passes <= 2ll * sms
-                     ? 1
-                     : (passes < kRopeUnroll ? passes : kRopeUnroll);
+  // kRopeUnroll, which spreads a row's sines over more of its heads. Of the
+  // upper half of the possible slot counts, the one that leaves the fewest
+  // heads' worth of threads idle (72 heads on 16 slots would run as 64 + 8).
+  int it = 1;
+  p.slots = most;
+  if (static_cast<long long>(rows) * ((total + most - 1) / most) > 2ll * sms) {
+    int least = 1 << 30;
+    for (int slots = most; slots > most / 2; --slots) {
+      const int passes = (total + slots - 1) / slots;
+      const int blocks = (passes + kRopeUnroll<INTER> - 1) / kRopeUnroll<INTER>;
+      const int per = (passes + blocks - 1) / blocks;
+      const int idle = slots * per * blocks - total;
+      if (idle < least) {
+        least = idle;
+        it = per;
+        p.slots = slots;
+      }
+    }
+  }
   p.heads_per_block = p.slots * it;
   const dim3 grid(rows, (total + p.heads_per_block - 1) / p.heads_per_block);
   const int threads = (p.slots * p.units + 31) / 32 * 32;
