@@ -114,7 +114,7 @@ struct RowParams {
   int whole;             // items are not cut
   const int* bt;
   const int* bt_off;
-  int block_size, box_rows, num_pages, layer;
+  int block_size, block_log2, box_rows, num_pages, layer;
   long long page_rows, layer_rows, kv_rows;  // strides in token slots
   float* ws_o;           // [2 * grid][256][128]
   float* ws_ml;          // [2 * grid][256][2]
@@ -170,6 +170,7 @@ __device__ __forceinline__ RowTables row_tables(uint8_t* smem) {
 __device__ __forceinline__ void build_prompt_tables(const RowParams& p, RowTables t,
                                                     int* scratch) {
   const int per = 2 * p.tile_tokens;
+#pragma unroll 1
   for (int s = threadIdx.x; s < p.S; s += kRowThreads) {
     const int a = p.q_off[s], b = p.q_off[s + 1];
     const bool bad = a < 0 || b < a || b > p.rows;
@@ -177,9 +178,11 @@ __device__ __forceinline__ void build_prompt_tables(const RowParams& p, RowTable
     scratch[s] = bad ? 0 : static_cast<int>((static_cast<long long>(b - a) + per - 1) / per);
   }
   __syncthreads();
+#pragma unroll 1
   for (int s = threadIdx.x; s < p.S; s += kRowThreads) {
     const int n = scratch[s];
     int rank = 0;
+#pragma unroll 1
     for (int i = 0; i < p.S; ++i) {
       const int m = scratch[i];
       rank += m > n || (m == n && i < s);
@@ -190,6 +193,7 @@ __device__ __forceinline__ void build_prompt_tables(const RowParams& p, RowTable
   __syncthreads();
   if (threadIdx.x < 32) {
     int before = 0;  // items of the ranks before this chunk
+#pragma unroll 1
     for (int r0 = 0; r0 < p.S; r0 += 32) {
       const int r = r0 + threadIdx.x;
       const int n = r < p.S ? t.count[r] : 0;
@@ -219,6 +223,7 @@ struct PromptItems {
     it.kh = w % p.HKV;
     const int u = w / p.HKV;
     int lo = 0, hi = p.S - 1;
+#pragma unroll 1
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (t.start[mid] <= u) lo = mid; else hi = mid - 1;
@@ -271,6 +276,7 @@ __device__ __forceinline__ int tree_tiles(const RowParams& p, int s, int& nodes,
 __device__ __forceinline__ void build_tree_tables(const RowParams& p, RowTables t, bool report) {
   if (threadIdx.x < 32) {
     int before = 0;
+#pragma unroll 1
     for (int s0 = 0; s0 < p.S; s0 += 32) {
       const int s = s0 + threadIdx.x;
       int n = 0;
@@ -309,6 +315,7 @@ struct TreeItems {
     }
     if (pos >= end) return false;
     int lo = 0, hi = p.S - 1;
+#pragma unroll 1
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (t.start[mid] <= pos) lo = mid; else hi = mid - 1;
@@ -351,6 +358,19 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
       : "memory");
 }
 
+// Bounded waits, counted in polls instead of by the clock: there are many of
+// them, and the kernel's code has to stay in the instruction cache.
+constexpr uint32_t kRowPolls = 1u << 26;  // of 20 ns and more: over a second
+__device__ __forceinline__ bool row_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+#pragma unroll 1
+  for (uint32_t left = kRowPolls; left != 0; --left) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((left & 63u) == 0 && *abort) return false;
+  }
+  *abort = 1;
+  return false;
+}
+
 // A count in shared memory that one warp raises and others wait for.
 __device__ __forceinline__ void st_release_cta(uint32_t* p, uint32_t v) {
   asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
@@ -362,42 +382,28 @@ __device__ __forceinline__ uint32_t ld_acquire_cta(const uint32_t* p) {
 }
 __device__ __forceinline__ bool count_wait(const uint32_t* p, uint32_t at_least,
                                            volatile int* abort) {
-  uint64_t t0 = 0;
-  for (uint32_t i = 0;; ++i) {
+#pragma unroll 1
+  for (uint32_t left = kRowPolls; left != 0; --left) {
     if (static_cast<int32_t>(ld_acquire_cta(p) - at_least) >= 0) return true;
-    if ((i & 255u) == 255u) {
-      if (*abort) return false;
-      const uint64_t now = globaltimer_ns();
-      if (t0 == 0) {
-        t0 = now;
-      } else if (now - t0 > kWaitTimeoutNs) {
-        *abort = 1;
-        return false;
-      }
-    }
+    if ((left & 255u) == 0 && *abort) return false;
   }
+  *abort = 1;
+  return false;
 }
 
 // A lock in shared memory between two threads of the CTA that each hold it
 // for a bounded time. Returns false when the wait gave up.
 __device__ __forceinline__ bool lock_take(uint32_t* p, volatile int* abort) {
-  uint64_t t0 = 0;
-  for (uint32_t i = 0;; ++i) {
+#pragma unroll 1
+  for (uint32_t left = kRowPolls; left != 0; --left) {
     uint32_t was;
-    asm volatile("atom.acquire.cta.shared::cta.cas.b32 %0, [%1], 0, 1;"
+    asm volatile("atom.relaxed.cta.shared::cta.cas.b32 %0, [%1], 0, 1;"
                  : "=r"(was) : "r"(smem_u32(p)) : "memory");
     if (was == 0) return true;
-    if ((i & 255u) == 255u) {
-      if (*abort) return false;
-      const uint64_t now = globaltimer_ns();
-      if (t0 == 0) {
-        t0 = now;
-      } else if (now - t0 > kWaitTimeoutNs) {
-        *abort = 1;
-        return false;
-      }
-    }
+    if ((left & 255u) == 0 && *abort) return false;
   }
+  *abort = 1;
+  return false;
 }
 
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
@@ -559,7 +565,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   // at the end, or when the wait gave up. A slot is given back by every user.
   auto next_item = [&](uint32_t ord, RowItem& it) {
     const uint32_t slot = ord % kRowItems;
-    if (!mbar_wait(&it_full[slot], (ord / kRowItems) & 1, abort_flag)) return false;
+    if (!row_wait(&it_full[slot], (ord / kRowItems) & 1, abort_flag)) return false;
     it = ring[slot];
     return it.n > 0;
   };
@@ -631,22 +637,25 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       RowItem it;
       uint32_t st = 0, phase = 1;  // the ring's next slot
       bool ok = true;
+#pragma unroll 1
       for (uint32_t ord = 0; ok && __all_sync(0xffffffffu, next_item(ord, it)); ++ord) {
         __syncwarp();
         if (lane == 0) item_done(ord);
         int have = -1;  // page ids [have, have + kPageSlots) of the sequence are in shared memory
+#pragma unroll 1
         for (int j = 0; j < it.n && ok; ++j) {
           const int k0 = (it.t0 + j) * 128;
           uint8_t* dst = tiles + st * L::kTile;
           if constexpr (TREE) {
             const int k1 = min(k0 + 128, it.keys);
-            const int pg0 = k0 / p.block_size, pg1 = (k1 - 1) / p.block_size;
+            const int pg0 = k0 >> p.block_log2, pg1 = (k1 - 1) >> p.block_log2;
             if (have < 0 || pg1 >= have + static_cast<int>(L::kPageSlots)) {
               have = pg0;
               const int bt0 = p.bt_off[it.s], bt_n = p.bt_off[it.s + 1] - bt0;
               const int last = min(have + static_cast<int>(L::kPageSlots),
-                                   (it.keys - 1) / p.block_size + 1);
+                                   ((it.keys - 1) >> p.block_log2) + 1);
               __syncwarp();
+#pragma unroll 1
               for (int i = have + lane; i < last; i += 32) {
                 const int page = i < bt_n ? p.bt[bt0 + i] : -1;
                 // Pages outside the pool or the table are reported and not
@@ -659,27 +668,27 @@ __global__ void __launch_bounds__(kRowThreads, 1)
               __syncwarp();
             }
             // lane i issues the boxes of the tile's i-th page
-            const int segs = (k1 - k0 + p.box_rows - 1) / p.box_rows;
+            const int segs = p.block_log2 >= 7 ? 1 : (k1 - k0 + p.box_rows - 1) >> p.block_log2;
             const int tok = k0 + lane * p.box_rows;
-            const int page = lane < segs ? page_ids[tok / p.block_size - have] : -1;
+            const int page = lane < segs ? page_ids[(tok >> p.block_log2) - have] : -1;
             const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
             bool got = true;
             if (lane == 0) {
-              got = mbar_wait(&empty[st], phase, abort_flag);
+              got = row_wait(&empty[st], phase, abort_flag);
               if (got) mbar_arrive_expect_tx(&full[st], boxes * p.box_rows * (D * 2u));
             }
             ok = __shfl_sync(0xffffffffu, got, 0);
             if (!ok) break;
             if (page >= 0) {
               const int row = static_cast<int>(page * p.page_rows + p.layer * p.layer_rows +
-                                               kv * p.kv_rows + tok % p.block_size);
+                                               kv * p.kv_rows + (tok & (p.block_size - 1)));
               dst += lane * p.box_rows * 128u;
 #pragma unroll
               for (int h = 0; h < L::kHalves; ++h)
                 tma_load_2d(dst + h * L::kHalf, map, &full[st], it.kh * D + h * 64, row);
             }
           } else if (lane == 0) {
-            if (!mbar_wait(&empty[st], phase, abort_flag)) {
+            if (!row_wait(&empty[st], phase, abort_flag)) {
               ok = false;
               break;
             }
@@ -702,12 +711,14 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         uint32_t uses0 = 0, uses1 = 0;
         const uint32_t bytes = L::kHalves * 64u * 2u * p.group * p.tile_tokens;
         bool ok = true;
+#pragma unroll 1
         for (uint32_t ord = 0; ok && next_item(ord, it); ++ord) {
           item_done(ord);
+#pragma unroll 1
           for (int x = 0; x < 2 && ok; ++x) {
             if (x == 1 && it.n1 == 0) break;
             uint32_t& uses = x ? uses1 : uses0;
-            if (!mbar_wait(&q_empty[x], (uses & 1) ^ 1, abort_flag)) { ok = false; break; }
+            if (!row_wait(&q_empty[x], (uses & 1) ^ 1, abort_flag)) { ok = false; break; }
             ++uses;
             mbar_arrive_expect_tx(&q_full[x], bytes);
             for (int h = 0; h < L::kHalves; ++h)
@@ -721,12 +732,14 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       RowItem it;
       uint32_t c = 0;
       bool ok = true;
+#pragma unroll 1
       for (uint32_t ord = 0; ok && __all_sync(0xffffffffu, next_item(ord, it)); ++ord) {
         const int dirty = first_dirty<TREE>(it);
         unsigned* bad = bad_words + (ord % kRowItems) * (kRowMaxDirty * 4);
+#pragma unroll 1
         for (int j = 0; j < it.n; ++j, ++c) {
           const uint32_t st = c % NV;
-          const bool in = mbar_wait(&v_full[st], (c / NV) & 1, abort_flag);
+          const bool in = row_wait(&v_full[st], (c / NV) & 1, abort_flag);
           if (!__all_sync(0xffffffffu, in)) { ok = false; break; }
           if (j >= dirty) {
             uint8_t* tile = smem + L::kOffV + st * L::kTile;
@@ -782,9 +795,10 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         // ---------------------------------------------- items
         Items items;
         RowItem it;
+#pragma unroll 1
         for (uint32_t ord = 0;; ++ord) {
           const uint32_t slot = ord % kRowItems;
-          if (!mbar_wait(&it_empty[slot], ((ord / kRowItems) & 1) ^ 1, abort_flag)) break;
+          if (!row_wait(&it_empty[slot], ((ord / kRowItems) & 1) ^ 1, abort_flag)) break;
           const bool more = items.next(p, tab, it);
           if (!more) it.n = 0;
           ring[slot] = it;
@@ -803,13 +817,14 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       uint32_t ord0 = 0, ord1 = 0;  // items before; those with a Q tile 1
       uint32_t tiles = 0, mine = 0;  // tiles and items of the stream before
       bool ok = true;
+#pragma unroll 1
       for (; ok && next_item(ord0, it); base += it.n, ++ord0, ord1 += it.n1 > 0) {
         item_done(ord0);
         const int cnt = it.count(x);
         const int qt = it.alt ? 0 : x;
         // Both streams look at Q tile 0 of every item, and both give it back:
         // neither can be a phase of any barrier ahead of the other's items.
-        if (!mbar_wait(&q_full[0], ord0 & 1, abort_flag)) break;
+        if (!row_wait(&q_full[0], ord0 & 1, abort_flag)) break;
         if (x == 1 && !it.alt) mbar_arrive(&q_empty[0]);
         const uint64_t q_desc = sdesc_sw128(smem_u32(smem + L::kOffQ + qt * L::kTile), 0, 1024);
         auto k_ready = [&](int i) {
@@ -819,8 +834,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         // K of the stream's i-th tile (and its Q tile) are in shared memory.
         auto wait_k = [&](int i) {
           const uint32_t g = base + it.tile(x, i);
-          return (i > 0 || !qt || mbar_wait(&q_full[1], ord1 & 1, abort_flag)) &&
-                 mbar_wait(&k_full[g % NK], (g / NK) & 1, abort_flag);
+          return (i > 0 || !qt || row_wait(&q_full[1], ord1 & 1, abort_flag)) &&
+                 row_wait(&k_full[g % NK], (g / NK) & 1, abort_flag);
         };
         if (cnt == 0) continue;
         // Step i issues P V of tile i - 1 and S of tile i together: the streams'
@@ -828,13 +843,14 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         // other's products, instead of both at half speed side by side. Only
         // when K of tile i is not there yet, P V goes ahead alone.
         bool held = false;
+#pragma unroll 1
         for (int i = 0; i <= cnt; ++i) {
           if (i > 0) {
             const int j = it.tile(x, i - 1);
             const uint32_t st = (base + j) % NV;
             if (!count_wait(v_count, base + j + 1, abort_flag) ||
-                (i == 1 && !mbar_wait(&o_free[x], (mine & 1) ^ 1, abort_flag)) ||
-                !mbar_wait(&p_full[x], tiles & 1, abort_flag)) {
+                (i == 1 && !row_wait(&o_free[x], (mine & 1) ^ 1, abort_flag)) ||
+                !row_wait(&p_full[x], tiles & 1, abort_flag)) {
               ok = false;
               break;
             }
@@ -884,7 +900,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       // Every MMA issued above must finish before TMEM is released.
       mma_commit(&drain[x]);
       volatile int local_abort = 0;
-      mbar_wait(&drain[x], 0, &local_abort);
+      row_wait(&drain[x], 0, &local_abort);
     }
   } else {
     // ------------------------------------------------ softmax / epilogue
@@ -899,6 +915,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     RowItem it;
     uint32_t tiles = 0, mine = 0, act1 = 0, alts = 0, ord = 0;
     bool ok = true;
+#pragma unroll 1
     for (; ok && __all_sync(0xffffffffu, next_item(ord, it)); ++ord) {
       const int cnt = it.count(x);
       if (cnt == 0) {
@@ -913,8 +930,9 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         mask = p.mask + static_cast<long long>(p.q_off[it.s] + min(token, it.nodes - 1)) * p.words;
       float m = -INFINITY, msl = 0.f;
       float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
       for (int i = 0; i < cnt; ++i) {
-        const bool ready = mbar_wait(&s_full[x], tiles & 1, abort_flag);
+        const bool ready = row_wait(&s_full[x], tiles & 1, abort_flag);
         ++tiles;
         if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
         tc_fence_after();
@@ -1006,13 +1024,13 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         continue;
       }
       // ---- epilogue
-      bool fin = mbar_wait(&o_full[x], mine & 1, abort_flag);
+      bool fin = row_wait(&o_full[x], mine & 1, abort_flag);
       float a0 = 1.f, a1 = 0.f;                  // weights of the two streams' O
       float ml = m == -INFINITY ? m : msl;       // running max, log2 units
       if (it.alt) {
         // (stream 1's statistics first: by then its earlier items are through)
-        fin = fin && mbar_wait(&alt_ml[alts & 1], (alts >> 1) & 1, abort_flag) &&
-              mbar_wait(&o_full[1], act1 & 1, abort_flag);
+        fin = fin && row_wait(&alt_ml[alts & 1], (alts >> 1) & 1, abort_flag) &&
+              row_wait(&o_full[1], act1 & 1, abort_flag);
         if (__all_sync(0xffffffffu, fin)) {
           const float2 o = alt_buf[(alts & 1) * 128 + r];
           const float mm = max2(ml, o.x);
@@ -1024,7 +1042,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         }
         ++alts;
       }
-      fin = fin && mbar_wait(&looked[ord % kRowItems], (ord / kRowItems) & 1, abort_flag);
+      fin = fin && row_wait(&looked[ord % kRowItems], (ord / kRowItems) & 1, abort_flag);
       if (!__all_sync(0xffffffffu, fin)) { ok = false; break; }
       ++mine;
       act1 += it.count(1) > 0;
@@ -1038,6 +1056,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       const int dirty = first_dirty<TREE>(it);
       const int bad_n = min(max(it.n - dirty, 0), kRowMaxDirty) * 4;
       unsigned any_bad = 0;
+#pragma unroll 1
       for (int w = 0; w < bad_n; ++w) any_bad |= bad[w];
       float inv = 1.0f;
       uint8_t* stage = smem + L::kOffOut + warp * 2048;
@@ -1054,6 +1073,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         if constexpr (TREE) {
           if (l == 0.f) {  // a row that sees no key at all is zero
             bool sees = it.ctx > 0;
+#pragma unroll 1
             for (int w = 0; w < p.words && !sees; ++w)
               sees = tree_bits(mask, p.words, it.nodes, w * 32) != 0;
             if (!sees) inv = 0.f;
@@ -1112,7 +1132,9 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         // After the row's own stores: finite + infinity is infinity, and NaN
         // and opposite infinities come out as they should.
         __syncwarp();
+#pragma unroll 1
         for (int w = 0; valid && w < bad_n; ++w) {
+#pragma unroll 1
           for (unsigned b = bad[w]; b != 0; b &= b - 1) {
             const int k = (it.t0 + dirty) * 128 + w * 32 + __ffs(b) - 1;
             const uint16_t* vr = value_row<TREE>(p, it, D, k);

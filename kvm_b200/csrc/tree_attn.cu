@@ -186,7 +186,7 @@ extern "C" int kvm_sm100_attention_tree_paged(
   p.q_pos = q_positions; p.mask = mask; p.words = mask_words;
   p.max_nodes = max_q_rows; p.max_keys = max_keys; p.whole = cut.whole;
   p.bt = block_table; p.bt_off = bt_offsets;
-  p.block_size = bs; p.box_rows = bs < 128 ? bs : 128;
+  p.block_size = bs; p.block_log2 = __builtin_ctz(bs); p.box_rows = bs < 128 ? bs : 128;
   p.num_pages = L->num_pages; p.layer = L->layer;
   p.page_rows = L->page_stride / L->token_stride;
   p.layer_rows = L->layer_stride / L->token_stride;
