@@ -748,11 +748,11 @@ __global__ void __launch_bounds__(kRowThreads, 1)
               const int r = q * 32 + lane;
               const int key = (it.t0 + j) * 128 + r;
               bool found = false;
-#pragma unroll
+#pragma unroll 1
               for (int h = 0; h < L::kHalves; ++h) {
                 uint8_t* row = tile + h * L::kHalf + r * 128;
                 if (key >= it.keys) {
-#pragma unroll
+#pragma unroll 1
                   for (int ch = 0; ch < 8; ++ch)
                     *reinterpret_cast<uint4*>(row + ((ch ^ (r & 7)) << 4)) =
                         make_uint4(0, 0, 0, 0);
@@ -944,22 +944,19 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         const int k0 = (it.t0 + it.tile(x, i)) * 128;
         const bool masked = TREE ? k0 + 128 > it.ctx
                                  : k0 + 127 > it.tok0 + q_tile * p.tile_tokens;
-        if constexpr (TREE) {
-          if (masked) {
+        if (masked) {
 #pragma unroll
-            for (int c4 = 0; c4 < 4; ++c4) {
-              const unsigned bits = tree_bits(mask, p.words, it.nodes, k0 + c4 * 32 - it.ctx);
-#pragma unroll
-              for (int c = 0; c < 32; ++c)
-                if (!(bits >> c & 1u)) s[c4 * 32 + c] = -INFINITY;
+          for (int c4 = 0; c4 < 4; ++c4) {
+            unsigned bits;  // the keys the row sees
+            if constexpr (TREE) {
+              bits = tree_bits(mask, p.words, it.nodes, k0 + c4 * 32 - it.ctx);
+            } else {
+              const int lim = token - k0 - c4 * 32;
+              bits = lim < 0 ? 0u : lim > 30 ? 0xffffffffu : (2u << lim) - 1u;
             }
-          }
-        } else {
-          if (masked) {
-            const int lim = token - k0;
 #pragma unroll
-            for (int c = 0; c < 128; ++c)
-              if (c > lim) s[c] = -INFINITY;
+            for (int c = 0; c < 32; ++c)
+              if (!(bits & (1u << c))) s[c4 * 32 + c] = -INFINITY;
           }
         }
         // Row max as four chains (max is exact in any order), two values a step.
@@ -1113,7 +1110,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                   stage + from * 64 + ((c ^ (from >> 1 & 3)) << 4));
           }
         };
-        if (it.part >= 0) {
+        if (TREE && it.part >= 0) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t w[16];
