@@ -66,6 +66,7 @@ constexpr int kRowMaxSeqs = 1024;       // sequences of one call (tables in shar
 constexpr int kRowMaxDirty = 10;        // V tiles of an item that a row sees in part
 constexpr int kRowItems = 4;            // item descriptions in the ring
 constexpr int kRowItemUsers = 14;       // warps that give one back: 0-12 and 14
+constexpr int kRowBadWords = kRowMaxDirty * 4 + 4;  // their bad values' keys; any; padding
 constexpr int kRowMaxNodes = 1024;
 
 // Shared memory of one CTA for head width D. ONE: no item has a second Q tile,
@@ -83,7 +84,7 @@ struct RowSmem {
   static constexpr uint32_t kOffTab = kOffV + kStagesV * kTile;
   static constexpr uint32_t kTabBytes = kRowMaxSeqs * (TREE ? 4 : 10) + 16;
   static constexpr uint32_t kOffBad = kOffTab + kTabBytes;
-  static constexpr uint32_t kOffItems = kOffBad + kRowItems * kRowMaxDirty * 16;
+  static constexpr uint32_t kOffItems = kOffBad + kRowItems * kRowBadWords * 4;
   static constexpr uint32_t kOffMl = kOffItems + kRowItems * 64;
   static constexpr uint32_t kOffPages = kOffMl + 2 * 128 * 8;
   static constexpr uint32_t kPageSlots = 128;                // page ids a producer reads ahead
@@ -416,6 +417,15 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
+__device__ __forceinline__ void st_global_if(bool on, unsigned long long to, uint4 v) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.u32 p, %0, 0;\n\t"
+      "@p st.global.v4.b32 [%1], {%2, %3, %4, %5};\n\t}" ::"r"(static_cast<uint32_t>(on)),
+      "l"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+      : "memory");
+}
+
 // 3-D tiled TMA load (x innermost).
 __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, uint64_t* bar,
                                             int32_t x, int32_t y, int32_t z) {
@@ -735,7 +745,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 #pragma unroll 1
       for (uint32_t ord = 0; ok && __all_sync(0xffffffffu, next_item(ord, it)); ++ord) {
         const int dirty = first_dirty<TREE>(it);
-        unsigned* bad = bad_words + (ord % kRowItems) * (kRowMaxDirty * 4);
+        unsigned any = 0;
+        unsigned* bad = bad_words + (ord % kRowItems) * kRowBadWords;
 #pragma unroll 1
         for (int j = 0; j < it.n; ++j, ++c) {
           const uint32_t st = c % NV;
@@ -776,6 +787,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                 }
               }
               const unsigned word = __ballot_sync(0xffffffffu, found);
+              any |= word;
               if (lane == 0 && j - dirty < kRowMaxDirty) bad[(j - dirty) * 4 + q] = word;
             }
             fence_async_smem();
@@ -786,6 +798,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         if (!ok) break;
         __syncwarp();
         if (lane == 0) {
+          bad[kRowMaxDirty * 4] = any;
           mbar_arrive(&looked[ord % kRowItems]);
           item_done(ord);
         }
@@ -1049,12 +1062,10 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       const int head = it.kh * p.group + r_head;
       // Values that are not finite, of keys this row sees (words of the item's
       // dirty tiles; all zero but for broken inputs).
-      const unsigned* bad = bad_words + (ord % kRowItems) * (kRowMaxDirty * 4);
+      const unsigned* bad = bad_words + (ord % kRowItems) * kRowBadWords;
       const int dirty = first_dirty<TREE>(it);
       const int bad_n = min(max(it.n - dirty, 0), kRowMaxDirty) * 4;
-      unsigned any_bad = 0;
-#pragma unroll 1
-      for (int w = 0; w < bad_n; ++w) any_bad |= bad[w];
+      const unsigned any_bad = bad[kRowMaxDirty * 4];
       float inv = 1.0f;
       uint8_t* stage = smem + L::kOffOut + warp * 2048;
       unsigned long long dst = 0;  // where the row goes
@@ -1065,6 +1076,13 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                   : reinterpret_cast<unsigned long long>(
                         static_cast<uint16_t*>(p.out) + row * p.ldo +
                         static_cast<long long>(head) * D);
+      // the pieces this lane stores: 16 bytes of the rows lane / 4 + 8 k
+      unsigned long long to[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        to[k] = __shfl_sync(0xffffffffu, dst, k * 8 + (lane >> 2));
+        if (to[k] != 0) to[k] += (lane & 3) * 16;
+      }
       if (it.part < 0) {
         inv = 1.0f / l;
         if constexpr (TREE) {
@@ -1101,14 +1119,15 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ (lane >> 1 & 3)) << 4)) =
                 make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
           __syncwarp();
+          uint4 v[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const int from = k * 8 + (lane >> 2), c = lane & 3;
-            const unsigned long long to = __shfl_sync(0xffffffffu, dst, from);
-            if (to != 0)
-              *reinterpret_cast<uint4*>(to + at + c * 16) = *reinterpret_cast<const uint4*>(
-                  stage + from * 64 + ((c ^ (from >> 1 & 3)) << 4));
+            const int from = k * 8 + (lane >> 2);
+            v[k] = *reinterpret_cast<const uint4*>(
+                stage + from * 64 + (((lane & 3) ^ (from >> 1 & 3)) << 4));
           }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) st_global_if(to[k] != 0, to[k] + at, v[k]);
         };
         if (TREE && it.part >= 0) {
 #pragma unroll
