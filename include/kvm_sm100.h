@@ -492,14 +492,15 @@ int kvm_sm100_kvcache_copy_pages(void* cache, const kvm_kv_layout* layout, int l
  * moves to position q_positions[s] + i, over `layers` layers from
  * layout->layer on, K and V: the accepted path of a drafted tree becomes the
  * sequence's next tokens. In place. A sequence whose list is not strictly
- * increasing, or with a position outside its table or a page outside the
- * pool, is left as it is and reported through the device status. The pages
+ * increasing, or with a position outside its table, a table outside the
+ * table_len entries of block_table or a page outside the pool, is left as it is and reported through the device status. The pages
  * moved to must not be shared between sequences of the call. No counterpart
  * in the reference (it has no tree decoding). */
 int kvm_sm100_kvcache_compact(void* cache, const kvm_kv_layout* layout, int layers,
                               const int32_t* kept, int n_kept, const int32_t* kept_offsets,
                               const int32_t* q_positions, const int32_t* block_table,
-                              const int32_t* bt_offsets, int S, kvm_stream_t stream);
+                              int table_len, const int32_t* bt_offsets, int S,
+                              kvm_stream_t stream);
 
 /* kernel.attn.decode (dialect.cpp:39) over the paged cache, causal: query
  * row r of sequence s (rows q_offsets[s]..) at position p = q_positions[s]
@@ -533,7 +534,8 @@ int kvm_sm100_attention_decode_paged(const void* q, int64_t ldq, const void* cac
  * sequences and 1024 nodes. max_q_rows and max_keys (cached tokens and nodes)
  * bound every sequence and size the workspace; a sequence beyond them, or
  * with bad offsets, is skipped and reported through the device status; so are
- * pages outside the pool, whose sequence's result is undefined. Slots past a
+ * pages outside the pool and positions outside a sequence's table or the
+ * table_len entries of block_table, whose sequence's result is undefined. Slots past a
  * sequence's last node and nodes a row does not see cannot reach it, NaN and
  * infinities included. */
 int64_t kvm_sm100_attention_tree_workspace(int S, int HQ, int HKV, int max_q_rows,
@@ -542,8 +544,8 @@ int kvm_sm100_attention_tree_paged(const void* q, int64_t ldq, const void* cache
                                    const kvm_kv_layout* layout, void* out, int64_t ldo,
                                    const int32_t* q_offsets, const int32_t* q_positions,
                                    const uint32_t* mask, int mask_words,
-                                   const int32_t* block_table, const int32_t* bt_offsets,
-                                   int S, int rows, int HQ, int max_q_rows, int max_keys,
+                                   const int32_t* block_table, int table_len,
+                                   const int32_t* bt_offsets, int S, int rows, int HQ, int max_q_rows, int max_keys,
                                    float scale, void* workspace, int64_t workspace_bytes,
                                    kvm_stream_t stream);
 

@@ -114,13 +114,13 @@ SIGNATURES = {
     "kvm_sm100_attention_packed": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I, _I, _I,
                                         _I, _I, _I, _F, _P]),
     "kvm_sm100_attention_tree_workspace": (_I64, [_I, _I, _I, _I, _I]),
-    "kvm_sm100_attention_tree_paged": (_I, [_P, _I64, _P, _P, _P, _I64, _P, _P, _P, _I, _P, _P,
-                                            _I, _I, _I, _I, _I, _F, _P, _I64, _P]),
+    "kvm_sm100_attention_tree_paged": (_I, [_P, _I64, _P, _P, _P, _I64, _P, _P, _P, _I, _P, _I,
+                                            _P, _I, _I, _I, _I, _I, _F, _P, _I64, _P]),
     "kvm_sm100_rope_table": (_I, [_P, _P]),
     "kvm_sm100_rope": (_I, [_P, _P, _I64, _P, _I64, _I, _P, _I64, _P, _I64, _I, _I, _I, _I, _I,
                             _I, _P, _I, _P]),
     "kvm_sm100_kvcache_copy_pages": (_I, [_P, _P, _I, _P, _P, _I, _P]),
-    "kvm_sm100_kvcache_compact": (_I, [_P, _P, _I, _P, _I, _P, _P, _P, _P, _I, _P]),
+    "kvm_sm100_kvcache_compact": (_I, [_P, _P, _I, _P, _I, _P, _P, _P, _I, _P, _I, _P]),
     "kvm_sm100_attention_decode_workspace": (_I64, [_I, _I, _I, _I, _I]),
     "kvm_sm100_attention_decode_paged": (_I, [_P, _I64, _P, _P, _P, _I64, _P, _P, _P, _P,
                                               _I, _I, _I, _I, _F, _P, _I64, _P]),

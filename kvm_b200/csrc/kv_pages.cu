@@ -92,7 +92,8 @@ __global__ void __launch_bounds__(kCompactThreads)
     compact_kernel(uint4* __restrict__ pool, const __grid_constant__ kvm_kv_layout L,
                    int layers, const int* __restrict__ kept, int n_kept,
                    const int* __restrict__ kept_off, const int* __restrict__ q_pos,
-                   const int* __restrict__ bt, const int* __restrict__ bt_off, int* status) {
+                   const int* __restrict__ bt, int table_len, const int* __restrict__ bt_off,
+                   int* status) {
   __shared__ long long from[kCompactBatch], to[kCompactBatch];
   pdl_wait();
   pdl_trigger();
@@ -104,8 +105,9 @@ __global__ void __launch_bounds__(kCompactThreads)
     if (threadIdx.x == 0) atomicOr(status, kDevBadInput);
     return;
   }
-  const int p0 = q_pos[s], b0 = bt_off[s];
-  const long long slots = static_cast<long long>(bt_off[s + 1] - b0) * L.block_size;
+  const int p0 = q_pos[s], b0 = bt_off[s], b1 = bt_off[s + 1];
+  const long long slots =
+      b0 < 0 || b1 > table_len ? 0 : (static_cast<long long>(b1) - b0) * L.block_size;
   // page of a position, or -1
   auto page_of = [&](long long pos) {
     if (pos < 0 || pos >= slots) return -1;
@@ -201,11 +203,11 @@ extern "C" int kvm_sm100_kvcache_compact(void* cache, const kvm_kv_layout* L, in
                                          const int32_t* kept, int n_kept,
                                          const int32_t* kept_offsets,
                                          const int32_t* q_positions,
-                                         const int32_t* block_table,
+                                         const int32_t* block_table, int table_len,
                                          const int32_t* bt_offsets, int S,
                                          kvm_stream_t stream) {
   if (int rc = check_kv_layout(L)) return rc;
-  if (layers <= 0 || S < 0 || n_kept < 0 || !cache || !aligned16(cache))
+  if (layers <= 0 || S < 0 || n_kept < 0 || table_len < 0 || !cache || !aligned16(cache))
     return fail(KVM_ERR_INVALID_ARG, "kvcache_compact: bad argument");
   if (S == 0 || n_kept == 0) return KVM_OK;
   if (!kept || !kept_offsets || !q_positions || !block_table || !bt_offsets)
@@ -218,6 +220,6 @@ extern "C" int kvm_sm100_kvcache_compact(void* cache, const kvm_kv_layout* L, in
   KVM_CUDA_TRY(launch_ex(true, compact_kernel, dim3(static_cast<unsigned>(blocks)),
                          dim3(kCompactThreads), 0, static_cast<cudaStream_t>(stream),
                          static_cast<uint4*>(cache), *L, layers, kept, n_kept, kept_offsets,
-                         q_positions, block_table, bt_offsets, dev->status));
+                         q_positions, block_table, table_len, bt_offsets, dev->status));
   return KVM_OK;
 }

@@ -115,6 +115,7 @@ struct RowParams {
   int whole;             // items are not cut
   const int* bt;
   const int* bt_off;
+  int bt_len;            // entries of bt
   int block_size, block_log2, box_rows, num_pages, layer;
   long long page_rows, layer_rows, kv_rows;  // strides in token slots
   float* ws_o;           // [2 * grid][256][128]
@@ -507,14 +508,20 @@ __device__ __forceinline__ int first_dirty(const RowItem& it) {
   return max(0, (k >> 7) - it.t0);
 }
 
+// Pages in sequence s's table, none if it leaves the list.
+__device__ __forceinline__ int table_entries(const RowParams& p, int s) {
+  const int a = p.bt_off[s], b = p.bt_off[s + 1];
+  return a < 0 || b > p.bt_len ? 0 : b - a;
+}
+
 // Address of the value row of key k (the epilogue's rare path), or NULL.
 template <bool TREE>
 __device__ __forceinline__ const uint16_t* value_row(const RowParams& p, const RowItem& it,
                                                      int D, int k) {
   long long row = it.key0 + k;
   if constexpr (TREE) {
-    const int idx = k / p.block_size, b0 = p.bt_off[it.s];
-    const int page = idx < p.bt_off[it.s + 1] - b0 ? p.bt[b0 + idx] : -1;
+    const int idx = k >> p.block_log2, b0 = p.bt_off[it.s];
+    const int page = idx < table_entries(p, it.s) ? p.bt[b0 + idx] : -1;
     if (page < 0 || page >= p.num_pages) return nullptr;
     row = page * p.page_rows + p.layer * p.layer_rows + p.kv_rows + k % p.block_size;
   }
@@ -661,7 +668,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             const int pg0 = k0 >> p.block_log2, pg1 = (k1 - 1) >> p.block_log2;
             if (have < 0 || pg1 >= have + static_cast<int>(L::kPageSlots)) {
               have = pg0;
-              const int bt0 = p.bt_off[it.s], bt_n = p.bt_off[it.s + 1] - bt0;
+              const int bt0 = p.bt_off[it.s], bt_n = table_entries(p, it.s);
               const int last = min(have + static_cast<int>(L::kPageSlots),
                                    ((it.keys - 1) >> p.block_log2) + 1);
               __syncwarp();

@@ -130,11 +130,12 @@ extern "C" int64_t kvm_sm100_attention_tree_workspace(int S, int HQ, int HKV, in
 extern "C" int kvm_sm100_attention_tree_paged(
     const void* q, int64_t ldq, const void* cache, const kvm_kv_layout* L, void* out,
     int64_t ldo, const int32_t* q_offsets, const int32_t* q_positions, const uint32_t* mask,
-    int mask_words, const int32_t* block_table, const int32_t* bt_offsets, int S, int rows,
+    int mask_words, const int32_t* block_table, int table_len, const int32_t* bt_offsets, int S,
+    int rows,
     int HQ, int max_q_rows, int max_keys, float scale, void* workspace,
     int64_t workspace_bytes, kvm_stream_t stream) {
   if (int rc = check_kv_layout(L)) return rc;
-  if (S < 0 || rows < 0 || HQ <= 0 || L->width % 128 || HQ % (L->width / 128))
+  if (S < 0 || rows < 0 || table_len < 0 || HQ <= 0 || L->width % 128 || HQ % (L->width / 128))
     return fail(KVM_ERR_INVALID_ARG,
                 "attention_tree: head_dim 128, width = HKV*128, HQ a multiple of HKV");
   const int HKV = L->width / 128, group = HQ / HKV, bs = L->block_size;
@@ -185,7 +186,7 @@ extern "C" int kvm_sm100_attention_tree_paged(
   p.v = cache; p.ldv = L->token_stride;
   p.q_pos = q_positions; p.mask = mask; p.words = mask_words;
   p.max_nodes = max_q_rows; p.max_keys = max_keys; p.whole = cut.whole;
-  p.bt = block_table; p.bt_off = bt_offsets;
+  p.bt = block_table; p.bt_off = bt_offsets; p.bt_len = table_len;
   p.block_size = bs; p.block_log2 = __builtin_ctz(bs); p.box_rows = bs < 128 ? bs : 128;
   p.num_pages = L->num_pages; p.layer = L->layer;
   p.page_rows = L->page_stride / L->token_stride;

@@ -142,7 +142,7 @@ class PagedKVCache:
                 _list(bt_offsets, "bt_offsets", dev) != S + 1:
             raise ValueError("q_offsets and bt_offsets must have one more entry than "
                              "q_positions")
-        _list(block_table, "block_table", dev)
+        table = _list(block_table, "block_table", dev)
         if q.dim() != 2 or tree_mask.dim() != 2:
             raise ValueError("q and tree_mask must be 2-D")
         rows, words = q.shape[0], tree_mask.shape[1]
@@ -161,7 +161,7 @@ class PagedKVCache:
         _call_on(dev, "kvm_sm100_attention_tree_paged", q.data_ptr(), ldq,
                  self.pool.data_ptr(), C.byref(self.layout_struct(layer)), out.data_ptr(), ldo,
                  q_offsets.data_ptr(), q_positions.data_ptr(), tree_mask.data_ptr(), words,
-                 block_table.data_ptr(), bt_offsets.data_ptr(), S, rows, heads_q, max_q_rows,
+                 block_table.data_ptr(), table, bt_offsets.data_ptr(), S, rows, heads_q, max_q_rows,
                  max_keys, scale, workspace.data_ptr(), workspace.nbytes)
         return out
 
@@ -192,8 +192,8 @@ class PagedKVCache:
                 _list(bt_offsets, "bt_offsets", dev) != S + 1:
             raise ValueError("kept_offsets and bt_offsets must have one more entry than "
                              "q_positions")
-        _list(block_table, "block_table", dev)
+        table = _list(block_table, "block_table", dev)
         _call_on(dev, "kvm_sm100_kvcache_compact", self.pool.data_ptr(),
                  C.byref(self.layout_struct(0)), self.layers, kept.data_ptr(), n,
-                 kept_offsets.data_ptr(), q_positions.data_ptr(), block_table.data_ptr(),
+                 kept_offsets.data_ptr(), q_positions.data_ptr(), block_table.data_ptr(), table,
                  bt_offsets.data_ptr(), S)

@@ -161,3 +161,37 @@ def test_page_calls_refuse(cuda):
     c.copy_pages(one[:0], one[:0])
     c.compact(one[:0], _i32([0, 0], cuda), one, one, _i32([0, 1], cuda))
     ops.device_status()
+
+
+def test_compact_refuses_tables_outside_the_list(cuda):
+    c = _cache(cuda, pages=4, layers=1, block_size=16, heads_kv=1)
+    want = _view(c).clone()
+    for bt_off in ([0, 9], [-1, 1], [2, 1]):
+        c.compact(_i32([2], cuda), _i32([0, 1], cuda), _i32([3], cuda), _i32([0, 1], cuda),
+                  _i32(bt_off, cuda))
+        with pytest.raises(KvmError):
+            ops.device_status()
+        assert torch.equal(_view(c), want)
+
+
+def test_page_calls_in_a_graph(cuda):
+    """Captured calls follow the lists and positions they find at replay."""
+    c = _cache(cuda, pages=20, layers=2, block_size=16, heads_kv=2)
+    src, dst = _i32([0, 1], cuda), _i32([5, 6], cuda)
+    kept, off, ctx = _i32([1, 3, 0, 7], cuda), _i32([0, 2, 4], cuda), _i32([14, 3], cuda)
+    bt, bt_off = [8, 9, 10, 11], [0, 2, 4]
+    args = (kept, off, ctx, _i32(bt, cuda), _i32(bt_off, cuda))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.copy_pages(src, dst)
+        c.compact(*args)
+    for s, d, k, p in (([0, 1], [5, 6], [1, 3, 0, 7], [14, 3]),
+                       ([6, 6], [2, 19], [0, 9, 2, 3], [0, 20])):
+        src.copy_(torch.tensor(s)), dst.copy_(torch.tensor(d))
+        kept.copy_(torch.tensor(k)), ctx.copy_(torch.tensor(p))
+        want = _view(c).clone()
+        want[torch.tensor(d)] = want[torch.tensor(s)]
+        want = _compact_ref(c, want, [k[:2], k[2:]], p, bt, bt_off)
+        graph.replay()
+        ops.device_status()
+        assert torch.equal(_view(c), want)

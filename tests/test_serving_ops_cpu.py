@@ -124,10 +124,11 @@ def test_page_calls_refuse_without_a_gpu():
     assert copy(P, C.byref(wide), 1, P, P, 1, None) in (_lib.KVM_ERR_UNSUPPORTED,
                                                         _lib.KVM_ERR_CUDA)
     comp = lambda *a: _rc("kvcache_compact", *a)  # noqa: E731
-    assert comp(P, C.byref(L), 1, None, 1, P, P, P, P, 1, None) == INV
-    assert comp(P, C.byref(L), 1, P, -1, P, P, P, P, 1, None) == INV
-    assert comp(P + 8, C.byref(L), 1, P, 1, P, P, P, P, 1, None) == INV
-    assert comp(P, C.byref(L), 1, None, 0, None, None, None, None, 1, None) == _lib.KVM_OK
+    assert comp(P, C.byref(L), 1, None, 1, P, P, P, 4, P, 1, None) == INV
+    assert comp(P, C.byref(L), 1, P, -1, P, P, P, 4, P, 1, None) == INV
+    assert comp(P + 8, C.byref(L), 1, P, 1, P, P, P, 4, P, 1, None) == INV
+    assert comp(P, C.byref(L), 1, P, 1, P, P, P, -1, P, 1, None) == INV
+    assert comp(P, C.byref(L), 1, None, 0, None, None, None, 0, None, 1, None) == _lib.KVM_OK
 
 
 def test_tree_mask():
@@ -169,20 +170,21 @@ def test_attention_tree_refuses_without_a_gpu():
 
     def rc(layout=None, **at):
         L = _lib.KvLayout(*{**lay, **(layout or {})}.values())
-        args = [P, 1024, P, C.byref(L), P, 1024, P, P, P, 1, P, P, 2, 10, 8, 5, 100, 0.0, P,
+        args = [P, 1024, P, C.byref(L), P, 1024, P, P, P, 1, P, 9, P, 2, 10, 8, 5, 100, 0.0, P,
                 1 << 40, None]
         for i, v in at.items():
             args[int(i[1:])] = v
         return _rc("attention_tree_paged", *args)
-    assert rc(a3=None) == INV and rc(layout=dict(width=192)) == INV and rc(a14=7) == INV
+    assert rc(a3=None) == INV and rc(layout=dict(width=192)) == INV and rc(a15=7) == INV
     assert rc(layout=dict(block_size=8)) == UNS and rc(layout=dict(block_size=48)) == UNS
     assert rc(layout=dict(kv_stride=4096 + 8)) == INV
-    assert rc(a12=1025) == UNS and rc(a15=0) == INV and rc(a15=1025, a9=64) == INV
-    assert rc(a15=33) == INV and rc(a16=0) == INV and rc(a17=float("nan")) == INV
+    assert rc(a13=1025) == UNS and rc(a16=0) == INV and rc(a16=1025, a9=64) == INV
+    assert rc(a16=33) == INV and rc(a17=0) == INV and rc(a18=float("nan")) == INV
     assert rc(a0=None) == INV and rc(a4=P + 4) == INV and rc(a8=None) == INV and rc(a1=1000) == INV
-    assert rc(a18=None, a16=2000) == INV and rc(a19=100, a16=2000) == INV
+    assert rc(a19=None, a17=2000) == INV and rc(a20=100, a17=2000) == INV
     assert rc(layout=dict(num_pages=1 << 30, page_stride=1 << 20)) == UNS
-    assert rc(a12=0) == _lib.KVM_OK and rc(a13=0) == _lib.KVM_OK
+    assert rc(a13=0) == _lib.KVM_OK and rc(a14=0) == _lib.KVM_OK
+    assert rc(a11=-1) == INV
     ws = _lib.lib().kvm_sm100_attention_tree_workspace
     assert ws(0, 8, 2, 5, 100) == 0 and ws(2, 7, 2, 5, 100) == 0 and ws(2, 8, 2, 0, 100) == 0
     assert ws(2, 8, 2, 5, 1024) == 0      # four short items are not cut

@@ -215,6 +215,19 @@ def test_tree_bad_pages_are_reported(cuda):
         check(out[4:], ref[4:], mag[4:], 304)      # the other sequence is served
 
 
+def test_tree_tables_outside_the_list_are_reported(cuda):
+    c = Case(cuda, ctx=[100, 300], nodes=[4, 4], hq=4, hkv=1, bs=16, seed=31)
+    n = c.bt.numel()
+    first = c.bt_off.tolist()[1]
+    for off in ([-1, first, n], [first + 1, first, n]):
+        out = c.cache.tree_decode(c.layer, c.q, c.q_off, c.q_pos, c.mask, c.bt, _i32(off, cuda),
+                                  heads_q=4, max_q_rows=4, max_keys=304)
+        with pytest.raises(KvmError):
+            ops.device_status()
+        ref, mag = c.exact()
+        check(out[4:], ref[4:], mag[4:], 304)
+
+
 def test_tree_graph_and_two_streams(cuda):
     """A captured call follows contexts that change; two calls at once with a
     workspace each."""
