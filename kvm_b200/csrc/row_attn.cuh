@@ -74,6 +74,14 @@ constexpr int kRowMaxNodes = 1024;
 template <int D, bool TREE, bool ONE>
 struct RowSmem {
   static constexpr int kHalves = D / 64;
+  // A step's products go out under a lock, one stream's after the other's, in
+  // items of kLockTiles key tiles and more, where the tensor cores are nearly the
+  // bound (16383 tokens: 2.1 ms with, 2.50 without at 128-wide heads, 1.83 and
+  // 2.05 at 64); not in shorter ones, which wait for their softmax (40 short
+  // prompts of 64-wide heads: 87 us with, 81 without), nor for trees of one Q
+  // tile, which wait for memory (96 us with, 94 without).
+  static constexpr bool kLock = !ONE;
+  static constexpr int kLockTiles = 6;
   static constexpr uint32_t kHalf = 128 * 64 * 2;            // 128 rows x 64 columns
   static constexpr uint32_t kTile = kHalves * kHalf;
   static constexpr int kStagesK = D == 128 ? 2 : 4;
@@ -858,6 +866,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                  row_wait(&k_full[g % NK], (g / NK) & 1, abort_flag);
         };
         if (cnt == 0) continue;
+        const bool locked = L::kLock && it.n >= L::kLockTiles;
         // Step i issues P V of tile i - 1 and S of tile i together: the streams'
         // products then follow one another, and one's softmax runs under the
         // other's products, instead of both at half speed side by side. Only
@@ -876,7 +885,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             }
             ++tiles;
             const bool both = i < cnt && k_ready(i);
-            if (!lock_take(mma_lock, abort_flag)) { ok = false; break; }
+            if (locked && !lock_take(mma_lock, abort_flag)) { ok = false; break; }
             held = true;
             tc_fence_after();
             const uint64_t v_desc =
@@ -889,13 +898,16 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             if (!it.shared(j)) mma_commit(&v_empty[st]);
             if (i == cnt) mma_commit(&o_full[x]);
             if (!both) {
-              st_release_cta(mma_lock, 0);
+              if (locked) st_release_cta(mma_lock, 0);
               held = false;
             }
           }
           if (i < cnt) {
             if (!held) {
-              if (!wait_k(i) || !lock_take(mma_lock, abort_flag)) { ok = false; break; }
+              if (!wait_k(i) || (locked && !lock_take(mma_lock, abort_flag))) {
+                ok = false;
+                break;
+              }
               tc_fence_after();
             }
             const int j = it.tile(x, i);
@@ -911,7 +923,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             mma_commit(&k_empty[st]);
             if (!it.shared(j)) mma_commit(&k_empty[st]);
             if (i == cnt - 1) mma_commit(&q_empty[qt]);
-            st_release_cta(mma_lock, 0);
+            if (locked) st_release_cta(mma_lock, 0);
             held = false;
           }
         }
