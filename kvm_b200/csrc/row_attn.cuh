@@ -80,8 +80,12 @@ struct RowSmem {
   // 2.05 at 64); not in shorter ones, which wait for their softmax (40 short
   // prompts of 64-wide heads: 87 us with, 81 without), nor for trees of one Q
   // tile, which wait for memory (96 us with, 94 without).
-  static constexpr bool kLock = !ONE;
+  static constexpr bool kLock = !ONE && D == 128;
   static constexpr int kLockTiles = 6;
+  // TMEM columns: S_0 and S_1 (128 each), O_0 and O_1 (D each). With 64-wide
+  // heads P_0 and P_1 (64 each) have their own; with 128 they lie over S.
+  static constexpr bool kOwnP = D == 64;
+  static constexpr uint32_t kColO = 256, kColP = kOwnP ? 384 : 0, kStepP = kOwnP ? 64 : 128;
   static constexpr uint32_t kHalf = 128 * 64 * 2;            // 128 rows x 64 columns
   static constexpr uint32_t kTile = kHalves * kHalf;
   static constexpr int kStagesK = D == 128 ? 2 : 4;
@@ -99,8 +103,9 @@ struct RowSmem {
   static constexpr uint32_t kOffOut = kOffPages + 2 * kPageSlots * 4;  // [8 warps][32 rows][64 B]
   static constexpr uint32_t kOffBar = kOffOut + 8 * 2048;
   // q_full[2] q_empty[2] k_full[] k_empty[] v_full[] v_empty[] s_full[2] p_full[2]
-  // o_full[2] o_free[2] alt_ml[2] looked[I] it_full[I] it_empty[I] drain[2]
-  static constexpr int kBars = 2 * (kStagesK + kStagesV) + 16 + 3 * kRowItems;
+  // o_full[2] o_free[2] alt_ml[2] looked[I] it_full[I] it_empty[I] drain[2] s_read[2]
+  // pv_done[2]
+  static constexpr int kBars = 2 * (kStagesK + kStagesV) + 20 + 3 * kRowItems;
   static constexpr size_t bytes() { return 1024 + kOffBar + kBars * 8 + 16; }
 };
 
@@ -576,6 +581,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   uint64_t* it_full = looked + kRowItems;       // [kRowItems]
   uint64_t* it_empty = it_full + kRowItems;     // [kRowItems] kRowItemUsers arrivals
   uint64_t* drain = it_empty + kRowItems;       // [2]
+  uint64_t* s_read = drain + 2;                 // [2] 128 arrivals (kOwnP)
+  uint64_t* pv_done = s_read + 2;               // [2] (kOwnP)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint32_t* v_count = tmem_slot + 2;            // V tiles looked over, ever
@@ -607,6 +614,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 2 - i);
       mbar_init(&drain[i], 1);
+      mbar_init(&s_read[i], 128);
+      mbar_init(&pv_done[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 128);
       mbar_init(&o_full[i], 1);
@@ -645,7 +654,6 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // columns: S_0 (P_0 over its first half), S_1, O_0, O_1
   const uint32_t tmem = *tmem_slot;
 
   if (warp >= 8) {
@@ -839,7 +847,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       constexpr uint32_t kIdescQK = row_idesc<F16>(128, 0);
       constexpr uint32_t kIdescPV = row_idesc<F16>(D, 1);
       const int x = warp - 8;
-      const uint32_t tS = tmem + x * 128, tO = tmem + 256 + x * 128;
+      const uint32_t tS = tmem + x * 128, tO = tmem + L::kColO + x * D;
+      const uint32_t tP = tmem + L::kColP + x * L::kStepP;
       RowItem it;
       uint32_t base = 0;          // key tiles of the items before
       uint32_t ord0 = 0, ord1 = 0;  // items before; those with a Q tile 1
@@ -871,45 +880,13 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         // products then follow one another, and one's softmax runs under the
         // other's products, instead of both at half speed side by side. Only
         // when K of tile i is not there yet, P V goes ahead alone.
-        bool held = false;
+        bool held = false, ahead = false;
 #pragma unroll 1
         for (int i = 0; i <= cnt; ++i) {
-          if (i > 0) {
-            const int j = it.tile(x, i - 1);
-            const uint32_t st = (base + j) % NV;
-            if (!count_wait(v_count, base + j + 1, abort_flag) ||
-                (i == 1 && !row_wait(&o_free[x], (mine & 1) ^ 1, abort_flag)) ||
-                !row_wait(&p_full[x], tiles & 1, abort_flag)) {
-              ok = false;
-              break;
-            }
-            ++tiles;
-            const bool both = i < cnt && k_ready(i);
-            if (locked && !lock_take(mma_lock, abort_flag)) { ok = false; break; }
-            held = true;
-            tc_fence_after();
-            const uint64_t v_desc =
-                sdesc_sw128(smem_u32(smem + L::kOffV + st * L::kTile), L::kHalf, 1024);
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-              mma_f16_ts(tO, tS + kk * 8, v_desc + kk * (2048 >> 4), kIdescPV,
-                         (i > 1 || kk > 0) ? 1u : 0u);
-            mma_commit(&v_empty[st]);
-            if (!it.shared(j)) mma_commit(&v_empty[st]);
-            if (i == cnt) mma_commit(&o_full[x]);
-            if (!both) {
-              if (locked) st_release_cta(mma_lock, 0);
-              held = false;
-            }
-          }
-          if (i < cnt) {
-            if (!held) {
-              if (!wait_k(i) || (locked && !lock_take(mma_lock, abort_flag))) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-            }
+          // Products of step i: with P in its own columns S of tile i, as soon as
+          // the scores of tile i - 1 have been read, then P V of tile i - 1; with P
+          // over S first P V, then S. `ahead`: S of tile i has gone out already.
+          auto issue_s = [&]() {
             const int j = it.tile(x, i);
             const uint32_t st = (base + j) % NK;
             const uint64_t k_desc = sdesc_sw128(smem_u32(smem + L::kOffK + st * L::kTile), 0, 1024);
@@ -923,6 +900,54 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             mma_commit(&k_empty[st]);
             if (!it.shared(j)) mma_commit(&k_empty[st]);
             if (i == cnt - 1) mma_commit(&q_empty[qt]);
+          };
+          ahead = false;
+          if (i > 0) {
+            const int j = it.tile(x, i - 1);
+            const uint32_t st = (base + j) % NV;
+            if (L::kOwnP && i < cnt) {
+              if (!row_wait(&s_read[x], tiles & 1, abort_flag)) { ok = false; break; }
+              if (k_ready(i)) {
+                tc_fence_after();
+                issue_s();
+                ahead = true;
+              }
+            }
+            if (!count_wait(v_count, base + j + 1, abort_flag) ||
+                (i == 1 && !row_wait(&o_free[x], (mine & 1) ^ 1, abort_flag)) ||
+                !row_wait(&p_full[x], tiles & 1, abort_flag)) {
+              ok = false;
+              break;
+            }
+            ++tiles;
+            const bool both = !L::kOwnP && i < cnt && k_ready(i);
+            if (locked && !lock_take(mma_lock, abort_flag)) { ok = false; break; }
+            held = true;
+            tc_fence_after();
+            const uint64_t v_desc =
+                sdesc_sw128(smem_u32(smem + L::kOffV + st * L::kTile), L::kHalf, 1024);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+              mma_f16_ts(tO, tP + kk * 8, v_desc + kk * (2048 >> 4), kIdescPV,
+                         (i > 1 || kk > 0) ? 1u : 0u);
+            mma_commit(&v_empty[st]);
+            if (!it.shared(j)) mma_commit(&v_empty[st]);
+            if (L::kOwnP) mma_commit(&pv_done[x]);
+            if (i == cnt) mma_commit(&o_full[x]);
+            if (!both) {
+              if (locked) st_release_cta(mma_lock, 0);
+              held = false;
+            }
+          }
+          if (i < cnt && !ahead) {
+            if (!held) {
+              if (!wait_k(i) || (locked && !lock_take(mma_lock, abort_flag))) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+            }
+            issue_s();
             if (locked) st_release_cta(mma_lock, 0);
             held = false;
           }
@@ -941,7 +966,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     const int quarter = warp & 3;               // TMEM lane quarter
     const int r = quarter * 32 + lane;          // row of the Q tile
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t tS = tmem + x * 128 + lanes, tP = tS, tO = tmem + 256 + x * 128 + lanes;
+    const uint32_t tS = tmem + x * 128 + lanes, tO = tmem + L::kColO + x * D + lanes;
+    const uint32_t tP = tmem + L::kColP + x * L::kStepP + lanes;
     const float sl2 = p.scale_log2;
     const int r_tok = r / p.group, r_head = r - r_tok * p.group;
     RowItem it;
@@ -973,6 +999,10 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         for (int c4 = 0; c4 < 4; ++c4)
           tmem_ld32(tS + c4 * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c4 * 32]));
         tmem_wait_ld();
+        if (L::kOwnP) {
+          tc_fence_before();
+          mbar_arrive(&s_read[x]);
+        }
         const int k0 = (it.t0 + it.tile(x, i)) * 128;
         const bool masked = TREE ? k0 + 128 > it.ctx
                                  : k0 + 127 > it.tok0 + q_tile * p.tile_tokens;
@@ -1000,6 +1030,11 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 #pragma unroll
         for (int u = 0; u < 4; ++u) mx[u] = max2(mx[u], s[124 + u]);
         const float mt = max2(max3(mx[0], mx[1], mx[2]), mx[3]);
+        if (L::kOwnP && tiles > 1) {  // the tile before has left P and reached O
+          const bool free = row_wait(&pv_done[x], tiles & 1, abort_flag);
+          if (!__all_sync(0xffffffffu, free)) { ok = false; break; }
+          tc_fence_after();
+        }
         if (i == 0) {
           m = mt;
           msl = m == -INFINITY ? 0.f : m * sl2;
@@ -1123,7 +1158,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 #pragma unroll
         for (int q = 0; q < 32; ++q) o[q] = __uint_as_float(u[q]);
         if (it.alt) {
-          tmem_ld32(tO + 128 + c4 * 32, u);
+          tmem_ld32(tO + D + c4 * 32, u);
           tmem_wait_ld();
 #pragma unroll
           for (int q = 0; q < 32; ++q) o[q] = o[q] * a0 + __uint_as_float(u[q]) * a1;
