@@ -385,8 +385,9 @@ int kvm_sm100_attention_prefill_bf16(const void* q, int64_t ldq, const void* k,
  * nor written. Softmax statistics and sums are fp32, P is rounded to dtype
  * for the product with V. What a row does not see (later rows, other
  * sequences) cannot reach it, NaN and infinities included. A sequence whose
- * offsets are descending or outside [0, rows] is skipped and reported through
- * the device status. No workspace. kernel.attn.prefill with the row offsets of
+ * offsets are descending or outside [0, rows] is left out, with all after it, and
+ * reported through the device status. scale <= 0 selects 1/sqrt(head_dim). No
+ * workspace. kernel.attn.prefill with the row offsets of
  * an attn_meta value (src/ir/dialect/kernel/values.h:83-117). */
 int kvm_sm100_attention_packed(const void* q, int64_t ldq, const void* k, int64_t ldk,
                                const void* v, int64_t ldv, void* out, int64_t ldo,
@@ -475,7 +476,8 @@ int kvm_sm100_kvcache_read(const void* cache, const kvm_kv_layout* layout, void*
                            const int32_t* bt_offsets, int S, int rows, kvm_stream_t stream);
 
 /* Page dst[i] of the pool := page src[i] for i < n, over `layers` layers from
- * layout->layer on, K and V (device lists of page ids). A source may repeat.
+ * layout->layer on (all of which the pool has), K and V (device lists of page
+ * ids). A source may repeat.
  * A pair whose page ids are out of range, whose destination another pair also
  * writes, or whose destination another pair reads is skipped and reported
  * through the device status, so the result does not depend on any order.

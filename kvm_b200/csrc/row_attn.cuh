@@ -10,8 +10,8 @@
 //
 //   warps 0-3, 4-7   softmax of stream 0 and 1, one thread per row: S row
 //                    from TMEM to registers, mask, running max m and sum l,
-//                    P = 2^(s - m) rounded to the input type over S's own
-//                    columns in TMEM; at the end O / l to global memory
+//                    P = 2^(s - m) rounded to the input type into TMEM; at the
+//                    end O / l to global memory
 //   warps 8, 9       MMA issuer (one lane) of stream 0 and 1: S_x = Q_x K_j^T
 //                    (shared memory operands), O_x += P_x V_j (P from TMEM:
 //                    shared memory carries Q, K and V reads only, 96 bytes a
@@ -30,17 +30,29 @@
 // with one thread issuing for both, its waits and commits (2000 cycles a
 // step) came between the products (16383 tokens of 32 + 4 heads: 2.97 ms).
 //
-// P overwrites S in place, so S_x(j+1) is issued after P V_x(j): MMAs of one
-// thread execute in order. For the same reason S_x(j+1) being complete means
-// that P V_x(j) is, and O_x may then be rescaled without another barrier. O
-// is rescaled only when a row's max grew by more than 2^8 since its P values
-// were scaled (P <= 2^8 is exact in range for bf16 and fp16, and l is fp32).
+// With 128-wide heads TMEM is full and P overwrites S in place, so S_x(j+1) is
+// issued after P V_x(j): MMAs of one thread execute in order. For the same
+// reason S_x(j+1) being complete means that P V_x(j) is, and O_x may then be
+// rescaled without another barrier. With 64-wide heads P has its own columns:
+// S_x(j+1) goes out as soon as S_x(j) has been read, under the powers (16383
+// tokens of 32 + 4 heads: 1.81 -> 1.58 ms), and a barrier tells when P V_x(j)
+// is done. O is rescaled only when a row's max grew by more than 2^8 since its
+// P values were scaled (P <= 2^8 is exact in range for bf16 and fp16, and l is
+// fp32).
 //
 // Masked keys: scores are replaced, not added to, so NaN or infinite keys
 // cannot reach a row that does not see them. Values are different, as 0 * NaN
-// = NaN in the product: warp 11 zeroes what is not finite in V tiles that
+// = NaN in the product: warp 12 zeroes what is not finite in V tiles that
 // some row sees only in part (and rows past the sequence's end), and the
 // epilogue adds those elements to the rows that do see them.
+//
+// Measured (B200): 16383 tokens of 32 + 4 heads of 128 in 2.0-2.26 ms, 975 to
+// 1090 TFLOP/s of causal products, of 1641 that cuBLAS reaches in a burst and
+// 1388 under the power cap; 32 trees of 16 nodes over 2000-4096 keys in 94-104
+// us, 3.9-4.3 TB/s of K and V. What bounds it is the chain of a stream's scores,
+// softmax and products (1950 cycles of softmax and as many of waiting a tile),
+// for trees the K/V tiles in flight. The code is kept short (waits counted in
+// polls, loops rolled): at 106 KB a sixth of its instruction requests missed.
 //
 // Every wait is bounded; a timeout sets the device status and the kernel
 // drains.
@@ -76,10 +88,9 @@ struct RowSmem {
   static constexpr int kHalves = D / 64;
   // A step's products go out under a lock, one stream's after the other's, in
   // items of kLockTiles key tiles and more, where the tensor cores are nearly the
-  // bound (16383 tokens: 2.1 ms with, 2.50 without at 128-wide heads, 1.83 and
-  // 2.05 at 64); not in shorter ones, which wait for their softmax (40 short
-  // prompts of 64-wide heads: 87 us with, 81 without), nor for trees of one Q
-  // tile, which wait for memory (96 us with, 94 without).
+  // bound (16383 tokens: 2.1 ms with, 2.50 without); not in shorter ones, which
+  // wait for their softmax, nor for trees of one Q tile, which wait for memory
+  // (32 trees: 96 us with, 94 without), nor where S does not wait for P V.
   static constexpr bool kLock = !ONE && D == 128;
   static constexpr int kLockTiles = 6;
   // TMEM columns: S_0 and S_1 (128 each), O_0 and O_1 (D each). With 64-wide
@@ -185,13 +196,23 @@ __device__ __forceinline__ RowTables row_tables(uint8_t* smem) {
 __device__ __forceinline__ void build_prompt_tables(const RowParams& p, RowTables t,
                                                     int* scratch) {
   const int per = 2 * p.tile_tokens;
+  // Sequences before the first bad one are disjoint, which bounds the items;
+  // the bad one and all after it are left out.
+  int* good = t.total;
+  if (threadIdx.x == 0) *good = p.S;
+  __syncthreads();
 #pragma unroll 1
   for (int s = threadIdx.x; s < p.S; s += kRowThreads) {
     const int a = p.q_off[s], b = p.q_off[s + 1];
     const bool bad = a < 0 || b < a || b > p.rows;
-    if (bad && blockIdx.x == 0) atomicOr(p.status, kDevBadInput);
+    if (bad) atomicMin(good, s);
     scratch[s] = bad ? 0 : static_cast<int>((static_cast<long long>(b - a) + per - 1) / per);
   }
+  __syncthreads();
+  const int n_good = *good;
+  if (n_good < p.S && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(p.status, kDevBadInput);
+#pragma unroll 1
+  for (int s = n_good + threadIdx.x; s < p.S; s += kRowThreads) scratch[s] = 0;
   __syncthreads();
 #pragma unroll 1
   for (int s = threadIdx.x; s < p.S; s += kRowThreads) {

@@ -121,7 +121,7 @@ using namespace kvm;
 extern "C" int64_t kvm_sm100_attention_tree_workspace(int S, int HQ, int HKV, int max_q_rows,
                                                       int max_keys) {
   if (S <= 0 || HQ <= 0 || HKV <= 0 || HQ % HKV || HQ / HKV > 128 || max_q_rows <= 0 ||
-      max_keys <= 0)
+      max_keys <= 0 || max_keys > (1 << 30))
     return 0;
   const TreeCut cut = tree_cut(S, HKV, HQ / HKV, max_q_rows, max_keys);
   return cut.whole ? 0 : cut.ctas * 2 * 256 * (128 + 2) * 4;
@@ -152,8 +152,9 @@ extern "C" int kvm_sm100_attention_tree_paged(
                 "attention_tree: page, layer and kv strides must be whole token slots");
   if (!std::isfinite(scale)) return fail(KVM_ERR_INVALID_ARG, "attention_tree: bad scale");
   if (S == 0 || rows == 0) return KVM_OK;
-  if (max_q_rows <= 0 || max_q_rows > kRowMaxNodes || max_keys <= 0)
-    return fail(KVM_ERR_INVALID_ARG, "attention_tree: max_q_rows 1..1024 and max_keys > 0");
+  if (max_q_rows <= 0 || max_q_rows > kRowMaxNodes || max_keys <= 0 || max_keys > (1 << 30))
+    return fail(KVM_ERR_INVALID_ARG,
+                "attention_tree: max_q_rows 1..1024 and max_keys 1..2^30");
   if (mask_words <= 0 || int64_t(mask_words) * 32 < max_q_rows)
     return fail(KVM_ERR_INVALID_ARG, "attention_tree: the mask holds fewer than max_q_rows bits");
   if (!q || !cache || !out || !q_offsets || !q_positions || !mask || !block_table ||

@@ -173,6 +173,14 @@ def test_packed_bad_offsets_are_reported(cuda):
         ops.device_status()
     check(out[:20], *(t[:20] for t in exact(q, k, v, [20], 2, 1, 128)), 20)
     assert bool((out[20:] == 3).all())
+    # what comes after a bad pair could cover rows twice: left out too
+    off = torch.tensor([0, 30, 10, 64], dtype=torch.int32, device=cuda)
+    out.fill_(3.0)
+    ops.attention_packed(q, k, v, off, heads_q=2, heads_kv=1, out=out)
+    with pytest.raises(KvmError):
+        ops.device_status()
+    check(out[:30], *(t[:30] for t in exact(q, k, v, [30], 2, 1, 128)), 30)
+    assert bool((out[30:] == 3).all())
 
 
 def test_packed_graph_and_stream(cuda):
