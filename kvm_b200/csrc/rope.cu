@@ -14,7 +14,7 @@
 // bits). One 64-bit multiply replaces a powf and a wide range reduction.
 //
 // Bound by HBM: every element is read once and written once (8192 rows of 72
-// heads of 128, bf16: 54.7 us interleaved, 5.5 TB/s; 64.9 us split). A block takes
+// heads of 128, bf16: 49.4 us interleaved, 6.1 TB/s; 47.7 us split). A block takes
 // one row and up to kRopeUnroll units a thread, whose loads are issued before
 // the row's d/2 sines are computed (one thread each, into shared memory) and
 // consumed after; a thread keeps the same columns in every head, so it reads
@@ -33,11 +33,10 @@ namespace kvm {
 namespace {
 
 constexpr int kRopeThreads = 256;
-// Units in flight per thread: 64 bytes of loads in either layout. (Four split
-// units take 106 registers; at two blocks an SM 8192 rows of 72 heads took 101
-// us instead of 58.)
-template <bool INTER>
-constexpr int kRopeUnroll = INTER ? 4 : 2;
+// Units in flight per thread: of 2, 3 and 4, 3 was the fastest in both layouts
+// (split, 8192 rows of 72 heads: 57.3, 47.7, 48.5 us), with at least 6 and 4
+// blocks an SM (interleaved with 4, 5, 6, 7: 51.9, 52.7, 49.4, 50.2 us).
+constexpr int kRopeUnroll = 3;
 
 struct RopeSide {
   const void* x;
@@ -67,6 +66,25 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float
   return __float2bfloat16_rn(v);
 }
 
+// Two neighbours at a time: one instruction packs both.
+__device__ __forceinline__ float2 load2(const __half* e) {
+  return __half22float2(*reinterpret_cast<const __half2*>(e));
+}
+__device__ __forceinline__ float2 load2(const __nv_bfloat16* e) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(e));
+}
+__device__ __forceinline__ float2 load2(const float* e) { return make_float2(e[0], e[1]); }
+__device__ __forceinline__ void store2(__half* e, float x, float y) {
+  *reinterpret_cast<__half2*>(e) = __floats2half2_rn(x, y);
+}
+__device__ __forceinline__ void store2(__nv_bfloat16* e, float x, float y) {
+  *reinterpret_cast<__nv_bfloat162*>(e) = __floats2bfloat162_rn(x, y);
+}
+__device__ __forceinline__ void store2(float* e, float x, float y) {
+  e[0] = x;
+  e[1] = y;
+}
+
 // V elements moved as one access when they fill 16 bytes, else one by one.
 template <typename T, int V>
 struct alignas(sizeof(T) * V == 16 ? 16 : alignof(T)) Vec {
@@ -76,7 +94,7 @@ struct alignas(sizeof(T) * V == 16 ? 16 : alignof(T)) Vec {
 // V: elements of a vector. Split layout: a rotating unit is the vectors at j
 // and j + rot/2; interleaved: one vector holding V/2 pairs.
 template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(kRopeThreads, 4)
+__global__ void __launch_bounds__(kRopeThreads, INTER ? 6 : 4)
     rope_rows_kernel(const __grid_constant__ RopeParams p,
                      const __grid_constant__ kvm_rope_table t) {
   __shared__ float2 cs[KVM_ROPE_MAX_PAIRS];
@@ -91,7 +109,7 @@ __global__ void __launch_bounds__(kRopeThreads, 4)
 
   pdl_wait();
   pdl_trigger();
-  constexpr int U = kRopeUnroll<INTER>;
+  constexpr int U = kRopeUnroll;
   W a[U], b[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -134,13 +152,27 @@ __global__ void __launch_bounds__(kRopeThreads, 4)
       T* y = static_cast<T*>(s.y) + row * s.ldy +
              static_cast<long long>(is_q ? h : h - p.q.heads) * p.head_dim + col;
       if (rotates) {
+        if constexpr (sizeof(T) * V == 16 && INTER) {
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          T& ra = INTER ? a[u].e[2 * i] : a[u].e[i];
-          T& rb = INTER ? a[u].e[2 * i + 1] : b[u].e[i];
+          for (int i = 0; i < NP; ++i) {
+            const float2 f = load2(a[u].e + 2 * i);
+            store2(a[u].e + 2 * i, f.x * w[i].x - f.y * w[i].y, f.y * w[i].x + f.x * w[i].y);
+          }
+        } else if constexpr (sizeof(T) * V == 16) {
+#pragma unroll
+          for (int i = 0; i < NP; i += 2) {
+            const float2 fa = load2(a[u].e + i), fb = load2(b[u].e + i);
+            store2(a[u].e + i, fa.x * w[i].x - fb.x * w[i].y,
+                   fa.y * w[i + 1].x - fb.y * w[i + 1].y);
+            store2(b[u].e + i, fb.x * w[i].x + fa.x * w[i].y,
+                   fb.y * w[i + 1].x + fa.y * w[i + 1].y);
+          }
+        } else {  // one pair
+          T& ra = a[u].e[0];
+          T& rb = INTER ? a[u].e[V - 1] : b[u].e[0];
           const float fa = to_f(ra), fb = to_f(rb);
-          ra = from_f<T>(fa * w[i].x - fb * w[i].y);
-          rb = from_f<T>(fb * w[i].x + fa * w[i].y);
+          ra = from_f<T>(fa * w[0].x - fb * w[0].y);
+          rb = from_f<T>(fb * w[0].x + fa * w[0].y);
         }
         *reinterpret_cast<W*>(y) = a[u];
         if (!INTER) *reinterpret_cast<W*>(y + half) = b[u];
@@ -177,7 +209,7 @@ cudaError_t rope_launch(RopeParams p, const kvm_rope_table& t, int rows, int sms
     int least = 1 << 30;
     for (int slots = most; slots > most / 2; --slots) {
       const int passes = (total + slots - 1) / slots;
-      const int blocks = (passes + kRopeUnroll<INTER> - 1) / kRopeUnroll<INTER>;
+      const int blocks = (passes + kRopeUnroll - 1) / kRopeUnroll;
       const int per = (passes + blocks - 1) / blocks;
       const int idle = slots * per * blocks - total;
       if (idle < least) {
