@@ -254,11 +254,15 @@ def lib() -> C.CDLL:
 
 def call(name: str, *args) -> None:
     """Call kvm_sm100_<name>; raise KvmError on a non-zero status."""
-    L = lib()
-    rc = getattr(L, name)(*args)
+    rc = getattr(lib(), name)(*args)
     if rc != KVM_OK:
-        msg = L.kvm_sm100_last_error()
-        raise KvmError(name, rc, msg.decode() if msg else "")
+        raise_status(name, rc)
+
+
+def raise_status(name: str, rc: int) -> None:
+    """Raise the KvmError of a call that returned the status `rc`."""
+    msg = lib().kvm_sm100_last_error()
+    raise KvmError(name, rc, msg.decode() if msg else "")
 
 
 def device_status(clear: bool = True) -> int:

@@ -59,6 +59,7 @@ class PagedKVCache:
         self.pages, self.layers, self.block_size = pages, layers, block_size
         self.heads_kv, self.width, self.layout = heads_kv, heads_kv * 128, layout
         self.strides = kv_strides(layout, pages, layers, block_size, self.width)
+        self._layouts: dict = {}
         n = pages * layers * 2 * block_size * self.width
         self.pool = torch.zeros(n, dtype=torch.bfloat16, device=device)
 
@@ -67,6 +68,13 @@ class PagedKVCache:
             raise ValueError("layer out of range")
         ps, ls, ks, ts = self.strides
         return _lib.KvLayout(ps, ls, ks, ts, self.block_size, layer, self.width, self.pages)
+
+    def _layout(self, layer: int):
+        """layout_struct(layer) by reference, made once per layer."""
+        ref = self._layouts.get(layer)
+        if ref is None:
+            ref = self._layouts[layer] = C.byref(self.layout_struct(layer))
+        return ref
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
               q_positions: torch.Tensor, block_table: torch.Tensor,
@@ -159,7 +167,7 @@ class PagedKVCache:
         elif workspace.get_device() != dev or not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous on the pool's device")
         _call_on(dev, "kvm_sm100_attention_tree_paged", q.data_ptr(), ldq,
-                 self.pool.data_ptr(), C.byref(self.layout_struct(layer)), out.data_ptr(), ldo,
+                 self.pool.data_ptr(), self._layout(layer), out.data_ptr(), ldo,
                  q_offsets.data_ptr(), q_positions.data_ptr(), tree_mask.data_ptr(), words,
                  block_table.data_ptr(), table, bt_offsets.data_ptr(), S, rows, heads_q, max_q_rows,
                  max_keys, scale, workspace.data_ptr(), workspace.nbytes)
@@ -176,7 +184,7 @@ class PagedKVCache:
         if _list(dst, "dst", dev) != n:
             raise ValueError("src and dst must have the same length")
         _call_on(dev, "kvm_sm100_kvcache_copy_pages", self.pool.data_ptr(),
-                 C.byref(self.layout_struct(0)), self.layers, src.data_ptr(), dst.data_ptr(), n)
+                 self._layout(0), self.layers, src.data_ptr(), dst.data_ptr(), n)
 
     def compact(self, kept: torch.Tensor, kept_offsets: torch.Tensor,
                 q_positions: torch.Tensor, block_table: torch.Tensor,
@@ -194,6 +202,6 @@ class PagedKVCache:
                              "q_positions")
         table = _list(block_table, "block_table", dev)
         _call_on(dev, "kvm_sm100_kvcache_compact", self.pool.data_ptr(),
-                 C.byref(self.layout_struct(0)), self.layers, kept.data_ptr(), n,
+                 self._layout(0), self.layers, kept.data_ptr(), n,
                  kept_offsets.data_ptr(), q_positions.data_ptr(), block_table.data_ptr(), table,
                  bt_offsets.data_ptr(), S)

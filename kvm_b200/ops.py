@@ -49,37 +49,40 @@ def _rowmajor(t: torch.Tensor, name: str) -> int:
 def _mat(t: torch.Tensor, name: str, dtype: torch.dtype, rows: int, cols: int,
          dev: int) -> int:
     """Checks a [rows, cols] matrix with contiguous rows on CUDA device `dev`;
-    returns its row stride. (One call per tensor: the small launches of a
-    decode step are bound by the host.)"""
+    returns its row stride. (The small launches of a decode step are bound by
+    the host: what passes is found out in few steps, what is wrong in others.)"""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev >= 0 and \
+            t.shape == (rows, cols):
+        stride = t.stride()
+        if stride[1] == 1 or cols <= 1:
+            return stride[0]
+        raise ValueError(f"{name} must have contiguous rows")
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype:
         raise TypeError(f"{name} must be a {dtype} tensor")
-    if t.get_device() != dev or dev < 0:
-        raise ValueError(f"{name} must be on the CUDA device of the call's other tensors "
-                         "(no CPU path exists)")
-    shape = t.shape
-    if len(shape) != 2 or shape[0] != rows or shape[1] != cols:
-        raise ValueError(f"{name} must be [{rows}, {cols}], got {tuple(shape)}")
-    stride = t.stride()
-    if stride[1] != 1 and cols > 1:
-        raise ValueError(f"{name} must have contiguous rows")
-    return stride[0]
+    if t.shape != (rows, cols):
+        raise ValueError(f"{name} must be [{rows}, {cols}], got {tuple(t.shape)}")
+    raise ValueError(f"{name} must be on the CUDA device of the call's other tensors "
+                     "(no CPU path exists)")
 
 
 def _list(t: torch.Tensor, name: str, dev: int, dtype: torch.dtype = torch.int32) -> int:
     """Checks a contiguous list on CUDA device `dev`; returns its length."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev >= 0 and \
+            t.dim() == 1 and t.is_contiguous():
+        return t.numel()
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype:
         raise TypeError(f"{name} must be a {dtype} tensor")
     if t.get_device() != dev or dev < 0:
         raise ValueError(f"{name} must be on the CUDA device of the call's other tensors")
-    if t.dim() != 1 or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous and 1-D")
-    return t.shape[0]
+    raise ValueError(f"{name} must be contiguous and 1-D")
 
 
 def _call_on(dev: int, name: str, *args) -> None:
     """call(name, *args, stream) with `dev` current and its current stream."""
     if torch._C._cuda_getDevice() == dev:
-        call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+        rc = getattr(_lib.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(dev))
+        if rc != _lib.KVM_OK:
+            _lib.raise_status(name, rc)
     else:
         with torch.cuda.device(dev):
             call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
