@@ -144,6 +144,15 @@ struct RowParams {
   long long page_rows, layer_rows, kv_rows;  // strides in token slots
   float* ws_o;           // [2 * grid][256][128]
   float* ws_ml;          // [2 * grid][256][2]
+  struct RowJoin* ws_join;  // [grid]
+};
+
+// What the joining kernel does for a CTA: the item that the CTA begins and the
+// next ones go on with (ntok0 = 0: none).
+struct RowJoin {
+  int row0, kh, ntok0, ntok1;
+  int part, last;        // the CTA's slot; the last CTA, which has its part in slot 2 * last
+  int s, tok0;
 };
 
 // A stretch of work: tiles [t0, t0 + n) of the keys for up to two Q tiles.
@@ -341,10 +350,11 @@ __device__ __forceinline__ int tree_share(int total, int ctas) {
 }
 
 struct TreeItems {
-  int pos = -1, end = 0, first = 1;
+  int pos = -1, end = 0, first = 1, share = 1;
   __device__ __forceinline__ bool next(const RowParams& p, const RowTables& t, RowItem& it) {
     if (pos < 0) {
-      const int total = *t.total, share = p.whole ? 1 : tree_share(total, gridDim.x);
+      const int total = *t.total;
+      share = p.whole ? 1 : tree_share(total, gridDim.x);
       const long long b = static_cast<long long>(blockIdx.x) * share;
       pos = b < total ? static_cast<int>(b) : total;
       end = min(pos + share, total);
@@ -857,6 +867,14 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           const uint32_t slot = ord % kRowItems;
           if (!row_wait(&it_empty[slot], ((ord / kRowItems) & 1) ^ 1, abort_flag)) break;
           const bool more = items.next(p, tab, it);
+          if constexpr (TREE) {
+            if (!p.whole && ord == 0) p.ws_join[blockIdx.x] = RowJoin{};  // none so far
+            if (more && it.part >= 0 && it.t0 == 0) {
+              const int end = items.pos - it.n + ((it.keys + 127) >> 7);
+              p.ws_join[blockIdx.x] = {it.row0, it.kh, it.ntok0, it.ntok1, it.part,
+                                       (end - 1) / items.share, it.s, it.tok0};
+            }
+          }
           if (!more) it.n = 0;
           ring[slot] = it;
           mbar_arrive(&it_full[slot]);
@@ -1007,6 +1025,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       const unsigned* mask = nullptr;
       if constexpr (TREE)  // rows past the tree's end read the last node's mask
         mask = p.mask + static_cast<long long>(p.q_off[it.s] + min(token, it.nodes - 1)) * p.words;
+      const bool counts = r_tok < (q_tile ? it.ntok1 : it.ntok0) && r_tok < p.tile_tokens;
       float m = -INFINITY, msl = 0.f;
       float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 1
@@ -1059,7 +1078,9 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         if (i == 0) {
           m = mt;
           msl = m == -INFINITY ? 0.f : m * sl2;
-        } else if (__any_sync(0xffffffffu, !((mt - m) * sl2 <= kRowRescale))) {
+        } else if (__any_sync(0xffffffffu, counts && !((mt - m) * sl2 <= kRowRescale))) {
+          // (rows of no token take no part in the vote: what they hold, and with it
+          // the roundings of the rows beside them, would differ from call to call)
           const float mn = max2(m, mt);
           const float nsl = mn == -INFINITY ? 0.f : mn * sl2;
           const float alpha = m == -INFINITY ? 0.f : ex2_approx(msl - nsl);
@@ -1132,7 +1153,6 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       ++mine;
       act1 += it.count(1) > 0;
       tc_fence_after();
-      const bool valid = r_tok < (q_tile ? it.ntok1 : it.ntok0) && r_tok < p.tile_tokens;
       const int row = it.row0 + q_tile * p.tile_tokens + r_tok;
       const int head = it.kh * p.group + r_head;
       // Values that are not finite, of keys this row sees (words of the item's
@@ -1144,7 +1164,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       float inv = 1.0f;
       uint8_t* stage = smem + L::kOffOut + warp * 2048;
       unsigned long long dst = 0;  // where the row goes
-      if (valid)
+      if (counts)
         dst = it.part >= 0
                   ? reinterpret_cast<unsigned long long>(
                         p.ws_o + (static_cast<long long>(it.part) * 256 + q_tile * 128 + r) * 128)
@@ -1224,7 +1244,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         // and opposite infinities come out as they should.
         __syncwarp();
 #pragma unroll 1
-        for (int w = 0; valid && w < bad_n; ++w) {
+        for (int w = 0; counts && w < bad_n; ++w) {
 #pragma unroll 1
           for (unsigned b = bad[w]; b != 0; b &= b - 1) {
             const int k = (it.t0 + dirty) * 128 + w * 32 + __ffs(b) - 1;
@@ -1244,7 +1264,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           }
         }
       }
-      if (it.part >= 0 && valid)
+      if (it.part >= 0 && counts)
         reinterpret_cast<float2*>(p.ws_ml)[static_cast<long long>(it.part) * 256 + q_tile * 128 +
                                            r] = make_float2(ml, l);
       tc_fence_before();

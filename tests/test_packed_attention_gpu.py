@@ -211,6 +211,19 @@ def test_packed_same_bits_every_time(cuda):
         assert torch.equal(a, ops.attention_packed(q, k, v, off, heads_q=16, heads_kv=2))
 
 
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 2, 128), (12, 4, 64), (5, 1, 128)])
+def test_packed_a_sequence_is_the_same_in_any_batch(cuda, hq, hkv, hd):
+    """Bit for bit: alone, and between others whose rows share its tiles."""
+    lens = [333, 50, 1, 700]
+    q, k, v, off = make(cuda, lens, hq, hkv, hd, torch.bfloat16, seed=11, std=3.0)
+    kw = dict(heads_q=hq, heads_kv=hkv, head_dim=hd)
+    out = ops.attention_packed(q, k, v, off, **kw)
+    for s in range(4):
+        r = slice(int(off[s]), int(off[s + 1]))
+        one = torch.tensor([0, lens[s]], dtype=torch.int32, device=cuda)
+        assert torch.equal(out[r], ops.attention_packed(q[r], k[r], v[r], one, **kw))
+
+
 def test_packed_refusals_and_empty(cuda):
     q, k, v, off = make(cuda, [8], 4, 2, 128, torch.bfloat16)
     kw = dict(heads_q=4, heads_kv=2)

@@ -190,5 +190,5 @@ def test_attention_tree_refuses_without_a_gpu():
     assert ws(2, 8, 2, 5, (1 << 30) + 1) == 0
     assert rc(a17=(1 << 30) + 1) == INV
     assert ws(2, 8, 2, 5, 1024) == 0      # four short items are not cut
-    assert ws(2, 8, 2, 5, 1025) == 9 * 2 * 256 * 130 * 4    # 36 key tiles, four to a CTA
-    assert ws(64, 64, 8, 16, 5000) == 148 * 2 * 256 * 130 * 4
+    assert ws(2, 8, 2, 5, 1025) == 9 * (2 * 256 * 130 * 4 + 32)    # 36 key tiles, four to a CTA
+    assert ws(64, 64, 8, 16, 5000) == 148 * (2 * 256 * 130 * 4 + 32)

@@ -188,6 +188,21 @@ def test_tree_scale_out_workspace_and_rows_left_alone(cuda):
         c.run(workspace=ws[:16], max_keys=2000)
 
 
+@pytest.mark.parametrize("i", [3, 5, 6, 8, 11])
+def test_tree_takes_nothing_from_the_workspace(cuda, i):
+    """Whatever an earlier call or another tensor left there."""
+    c = Case(cuda, seed=i, **CASES[i])
+    want = c.run()
+    n = c.cache.tree_workspace(len(c.ctx), heads_q=c.hq, max_q_rows=max(c.nodes),
+                               max_keys=max(a + b for a, b in zip(c.ctx, c.nodes)))
+    for fill in (0, 1, 0x7F, 0xFF):
+        ws = torch.full((n,), fill, dtype=torch.uint8, device=cuda)
+        assert torch.equal(c.run(workspace=ws), want)
+    ws.copy_(torch.randint(0, 256, (n,), device=cuda, dtype=torch.uint8))
+    assert torch.equal(c.run(workspace=ws), want)
+    ops.device_status()
+
+
 def test_tree_out_of_bounds_sequences_are_reported(cuda):
     """More nodes or keys than the bounds allow: that sequence is skipped."""
     for kw, skipped in ((dict(max_q_rows=5), 0), (dict(max_keys=200), 1)):
