@@ -48,8 +48,8 @@
 //
 // Measured (B200): 16383 tokens of 32 + 4 heads of 128 in 2.0-2.26 ms, 975 to
 // 1090 TFLOP/s of causal products, of 1641 that cuBLAS reaches in a burst and
-// 1388 under the power cap; 32 trees of 16 nodes over 2000-4096 keys in 94-104
-// us, 3.9-4.3 TB/s of K and V. What bounds it is the chain of a stream's scores,
+// 1388 under the power cap; 32 trees of 16 nodes over 2000-4096 keys in 86-95
+// us with the joins, 4.2-4.7 TB/s of K and V. What bounds it is the chain of a stream's scores,
 // softmax and products (1950 cycles of softmax and as many of waiting a tile),
 // for trees the K/V tiles in flight. The code is kept short (waits counted in
 // polls, loops rolled): at 106 KB a sixth of its instruction requests missed.
