@@ -376,18 +376,25 @@ int kvm_sm100_attention_prefill_bf16(const void* q, int64_t ldq, const void* k,
                                      void* workspace, int64_t workspace_bytes,
                                      kvm_stream_t stream);
 
-/* The same over packed sequences of different lengths: sequence s owns rows
- * offsets[s]..offsets[s+1] of q, k, v and out (device memory, S+1 entries;
- * lengths from 0 up, at most 1024 sequences), and row r attends to the rows
- * of its sequence up to itself. head_dim 64 or 128, dtype KVM_EW_BF16 or
- * KVM_EW_F16, at most 128 query heads per kv head; `rows` rows exist in the
- * tensors, and rows that belong to no sequence are neither read into a result
- * nor written. Softmax statistics and sums are fp32, P is rounded to dtype
- * for the product with V. What a row does not see (later rows, other
- * sequences) cannot reach it, NaN and infinities included. A sequence whose
- * offsets are descending or outside [0, rows] is left out, with all after it, and
- * reported through the device status. scale <= 0 selects 1/sqrt(head_dim). No
- * workspace. kernel.attn.prefill with the row offsets of
+/* The calls for serving - kvm_sm100_attention_packed here, and
+ * kvm_sm100_attention_tree_paged, kvm_sm100_kvcache_copy_pages,
+ * kvm_sm100_kvcache_compact and kvm_sm100_rope below - launch with programmatic
+ * dependent launch: a launch may start its prologue while the previous kernel on
+ * the stream finishes, and touches global memory only after that kernel has
+ * completed. Stream order is kept as for any launch. */
+
+/* Causal attention as above over packed sequences of different lengths:
+ * sequence s owns rows offsets[s]..offsets[s+1] of q, k, v and out (device
+ * memory, S+1 entries; lengths from 0 up, at most 1024 sequences), and row r
+ * attends to the rows of its sequence up to itself. head_dim 64 or 128, dtype
+ * KVM_EW_BF16 or KVM_EW_F16, at most 128 query heads per kv head; `rows` rows
+ * exist in the tensors, and rows that belong to no sequence are neither read
+ * into a result nor written. Softmax statistics and sums are fp32, P is
+ * rounded to dtype for the product with V. What a row does not see (later
+ * rows, other sequences) cannot reach it, NaN and infinities included. A
+ * sequence whose offsets are descending or outside [0, rows] is left out, with
+ * all after it, and reported through the device status. scale <= 0 selects
+ * 1/sqrt(head_dim). No workspace. kernel.attn.prefill with the row offsets of
  * an attn_meta value (src/ir/dialect/kernel/values.h:83-117). */
 int kvm_sm100_attention_packed(const void* q, int64_t ldq, const void* k, int64_t ldk,
                                const void* v, int64_t ldv, void* out, int64_t ldo,
