@@ -155,7 +155,7 @@ class PagedKVCache:
             raise ValueError("q and tree_mask must be 2-D")
         rows, words = q.shape[0], tree_mask.shape[1]
         ldq = _mat(q, "q", torch.bfloat16, rows, heads_q * 128, dev)
-        if _mat(tree_mask, "tree_mask", torch.int32, rows, words, dev) != words and rows > 1:
+        if _mat(tree_mask, "tree_mask", torch.int32, rows, words, dev) != words:
             raise ValueError("tree_mask must be contiguous")
         if out is None:
             out = torch.zeros((rows, heads_q * 128), dtype=q.dtype, device=q.device)

@@ -49,13 +49,14 @@ def _rowmajor(t: torch.Tensor, name: str) -> int:
 def _mat(t: torch.Tensor, name: str, dtype: torch.dtype, rows: int, cols: int,
          dev: int) -> int:
     """Checks a [rows, cols] matrix with contiguous rows on CUDA device `dev`;
-    returns its row stride. (The small launches of a decode step are bound by
+    returns its row stride, which for one row (torch leaves it free there) is
+    cols. (The small launches of a decode step are bound by
     the host: what passes is found out in few steps, what is wrong in others.)"""
     if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev >= 0 and \
             t.shape == (rows, cols):
         stride = t.stride()
         if stride[1] == 1 or cols <= 1:
-            return stride[0]
+            return stride[0] if rows > 1 else cols
         raise ValueError(f"{name} must have contiguous rows")
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype:
         raise TypeError(f"{name} must be a {dtype} tensor")

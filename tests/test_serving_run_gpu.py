@@ -171,3 +171,31 @@ def test_the_same_run_gives_the_same_bits(cuda):
             n.mul_(2.0)
         for a, b in zip(first, _run(cuda)):
             assert torch.equal(a, b)
+
+
+def test_one_row_has_no_row_stride(cuda):
+    """torch leaves the stride of a dimension of one entry free; the calls take
+    such a row, whatever its stride says, and give what they give for a plain one."""
+    def odd(x):
+        return x.as_strided(x.shape, (1, 1))
+    tok = Tokens(cuda, 1)
+    q, k, v = tok.q[0], tok.k[0], tok.v[0]
+    table, pos = ops.rope_table(HD), _i32([5], cuda)
+    kw = dict(heads=HQ, heads_kv=HKV)
+    outs = []
+    for f in (lambda x: x, odd):
+        rq, rk = ops.rope(f(q), pos, table, k=f(k), out=f(torch.empty_like(q)),
+                          out_k=f(torch.empty_like(k)), **kw)
+        a = ops.attention_packed(f(rq), f(rk), f(v), _i32([0, 1], cuda), heads_q=HQ,
+                                 heads_kv=HKV, out=f(torch.empty_like(q)))
+        cache = PagedKVCache(pages=1, layers=1, block_size=BS, heads_kv=HKV, device=cuda)
+        one, zero = _i32([0, 1], cuda), _i32([0], cuda)
+        cache.write(0, rk.view(-1)[None], v, one, zero, zero, one)
+        mask = torch.ones((1, 1), dtype=torch.int32, device=cuda)
+        b = cache.tree_decode(0, f(rq), one, zero, mask, zero, one, heads_q=HQ, max_q_rows=1,
+                              max_keys=1, out=f(torch.empty_like(q)))
+        outs.append([t.contiguous().view(-1) for t in (rq, rk, a, b)])
+    ops.device_status()
+    for x, y in zip(*outs):
+        assert torch.equal(x, y)
+    assert torch.equal(outs[0][2], v.view(HKV, 1, HD).expand(-1, HQ // HKV, -1).reshape(-1))
