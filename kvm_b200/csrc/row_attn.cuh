@@ -766,7 +766,10 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             phase ^= 1;
           }
         }
-        __syncwarp();
+        // Of prompts only lane 0 waits. When its wait gave up all lanes leave
+        // together: the others would be in the next vote without it for ever.
+        if constexpr (TREE) __syncwarp();
+        else ok = __shfl_sync(0xffffffffu, ok, 0) != 0;
       }
     } else if (warp == 11) {
       if (lane == 0) {
