@@ -541,10 +541,12 @@ int kvm_sm100_attention_decode_paged(const void* q, int64_t ldq, const void* cac
  * zeros. One node with bit 0 set is plain decoding. Heads and layout as for
  * kvm_sm100_attention_decode_paged, at most 128 query heads per kv head, 1024
  * sequences and 1024 nodes. max_q_rows and max_keys (cached tokens and nodes)
- * bound every sequence and size the workspace; a sequence beyond them, or
- * with bad offsets, is skipped and reported through the device status; so are
- * pages outside the pool and positions outside a sequence's table or the
- * table_len entries of block_table, whose sequence's result is undefined. Slots past a
+ * bound every sequence and size the workspace; a sequence beyond them, or at a
+ * negative position, is skipped and reported through the device status. One
+ * whose offsets are descending or outside [0, rows] is left out, with all after
+ * it (their rows could be another's), and reported. Pages outside the pool and
+ * positions outside a sequence's table or the table_len entries of block_table
+ * are reported, and that sequence's result is undefined. Slots past a
  * sequence's last node and nodes a row does not see cannot reach it, NaN and
  * infinities included. */
 int64_t kvm_sm100_attention_tree_workspace(int S, int HQ, int HKV, int max_q_rows,

@@ -305,31 +305,44 @@ __device__ __forceinline__ int tree_pairs(const RowParams& p, int nodes) {
   return (nodes + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
 }
 
+// Whether a sequence's rows [a, b) are no rows of q.
+__device__ __forceinline__ bool tree_bad_rows(const RowParams& p, int a, int b) {
+  return a < 0 || b < a || b > p.rows;
+}
+
 // Key tiles of sequence s, 0 for one that is empty or refused.
 __device__ __forceinline__ int tree_tiles(const RowParams& p, int s, int& nodes, int& ctx,
                                           bool report) {
   const int a = p.q_off[s], b = p.q_off[s + 1];
   ctx = p.q_pos[s];
   nodes = b - a;
-  const bool bad = a < 0 || b < a || b > p.rows || ctx < 0 || nodes > p.max_nodes ||
+  const bool bad = tree_bad_rows(p, a, b) || ctx < 0 || nodes > p.max_nodes ||
                    ctx > p.max_keys - nodes;
   if (bad && report) atomicOr(p.status, kDevBadInput);
   if (bad || nodes == 0) { nodes = 0; return 0; }
   return (ctx + nodes + 127) >> 7;
 }
 
+// Sequences before the first one with bad rows own disjoint rows; that one and
+// all after it are left out, as they could write rows of the others.
 __device__ __forceinline__ void build_tree_tables(const RowParams& p, RowTables t, bool report) {
   if (threadIdx.x < 32) {
     int before = 0;
+    bool left_out = false;  // by a sequence of an earlier chunk
 #pragma unroll 1
     for (int s0 = 0; s0 < p.S; s0 += 32) {
       const int s = s0 + threadIdx.x;
       int n = 0;
+      bool bad_rows = false;
       if (s < p.S) {
         int nodes, ctx;
         const int tiles = tree_tiles(p, s, nodes, ctx, report);
         n = (p.whole ? tiles > 0 : tiles) * tree_pairs(p, nodes) * p.HKV;
+        bad_rows = tree_bad_rows(p, p.q_off[s], p.q_off[s + 1]);
       }
+      const unsigned from = __ballot_sync(0xffffffffu, bad_rows);
+      if (left_out || (from & ((2u << threadIdx.x) - 1u)) != 0) n = 0;
+      left_out = left_out || from != 0;
       int sum = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {

@@ -217,6 +217,42 @@ def test_tree_out_of_bounds_sequences_are_reported(cuda):
         check(out[r[1 - skipped]], ref[r[1 - skipped]], mag[r[1 - skipped]], 404)
 
 
+@pytest.mark.parametrize("ctx", [[300, 40, 200], [5000, 40, 200]])     # whole items, cut ones
+def test_tree_after_bad_offsets_nothing_is_written(cuda, ctx):
+    """Rows of a sequence after a descending pair of offsets can be another
+    sequence's: that one keeps its result, the later ones are left out."""
+    c = Case(cuda, ctx=ctx, nodes=[9, 0, 4], hq=8, hkv=2, bs=16, seed=32)
+    ref, mag = c.exact()
+    for off, served in (([0, 9, 4, 13], 9), ([0, 9, 20, 13], 9), ([0, -1, 9, 13], 0),
+                        ([-4, 9, 9, 13], 0)):
+        for turn in range(5):
+            out = torch.full_like(c.q, 9.0)
+            c.cache.tree_decode(c.layer, c.q, _i32(off, cuda), c.q_pos, c.mask, c.bt, c.bt_off,
+                                heads_q=8, max_q_rows=9, max_keys=max(ctx) + 9, out=out)
+            with pytest.raises(KvmError):
+                ops.device_status()
+            check(out[:served], ref[:served], mag[:served], max(ctx) + 9)
+            assert bool((out[served:] == 9).all())
+
+
+def test_tree_bad_offsets_far_down_the_list(cuda):
+    """The first bad pair is the 36th of 70: the 35 before it are served."""
+    n = 70
+    c = Case(cuda, ctx=[(i * 13) % 90 for i in range(n)], nodes=[1 + i % 3 for i in range(n)],
+             hq=4, hkv=1, bs=16, seed=33)
+    off = c.off.copy()
+    off[36] = off[30]                            # sequence 35 descends, 36 covers rows of 30..36
+    out = torch.full_like(c.q, 9.0)
+    c.cache.tree_decode(c.layer, c.q, _i32(off, cuda), c.q_pos, c.mask, c.bt, c.bt_off, heads_q=4,
+                        max_q_rows=32, max_keys=130, out=out)
+    with pytest.raises(KvmError):
+        ops.device_status()
+    ref, mag = c.exact()
+    m = int(off[35])
+    check(out[:m], ref[:m], mag[:m], 95)
+    assert bool((out[m:] == 9).all())
+
+
 def test_tree_bad_pages_are_reported(cuda):
     c = Case(cuda, ctx=[100, 300], nodes=[4, 4], hq=4, hkv=1, bs=16, seed=25)
     for bad in (-1, 10 ** 6, c.cache.pages):
