@@ -100,6 +100,39 @@ def test_rope(cuda, dtype, inter, rows, heads, kvh, hd, rot, cfg):
     assert torch.equal(yq.cpu().double()[kept], ref[kept])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("heads,kvh,hd,rot", [
+    (64, 8, 128, 128),      # one to three blocks a row
+    (64, 8, 128, 64),
+    (37, 5, 128, 128),      # a last pass that is not full
+    (50, 3, 80, 32),
+    (31, 2, 96, 36),        # units of one pair, many blocks a row
+    (1, 70, 64, 64),        # the border of q and k within the first pass
+])
+def test_rope_many_rows(cuda, dtype, inter, heads, kvh, hd, rot):
+    """More rows than two blocks an SM, where blocks take their heads in two or
+    three passes; in place the same bits."""
+    rows = 300
+    g = torch.Generator(device="cuda").manual_seed(heads + hd + rot)
+    f, m = _freqs(rot, **YARN)
+    table = ops.rope_table(rot, **YARN)
+    qkv = torch.randn((rows, (heads + kvh) * hd + 8), generator=g, device=cuda).to(dtype)
+    q, k = qkv[:, :heads * hd], qkv[:, heads * hd:(heads + kvh) * hd]
+    pos = torch.randint(0, 100000, (rows,), generator=g, device=cuda)
+    kw = dict(heads=heads, head_dim=hd, interleaved=inter, k=k, heads_kv=kvh)
+    yq, yk = ops.rope(q, pos, table, **kw)
+    for got, x, n in ((yq, q, heads), (yk, k, kvh)):
+        ref, size = _ref(x, pos, n, hd, f, m, inter)
+        _close(got, ref, size)
+        kept = size == 0
+        assert torch.equal(got.cpu().double()[kept], ref[kept])
+    tail = qkv[:, (heads + kvh) * hd:].clone()
+    ops.rope(q, pos, table, out=q, out_k=k, **kw)
+    assert torch.equal(q, yq) and torch.equal(k, yk)
+    assert torch.equal(qkv[:, (heads + kvh) * hd:], tail)
+
+
 def test_rope_far_and_negative_positions(cuda):
     """int64 positions up to 2^40 and negative ones. The 64-bit reference angle
     is itself rounded (2^40 * 2^-53 = 2^-13), so the far rows are checked with
