@@ -391,8 +391,10 @@ int kvm_sm100_attention_prefill_bf16(const void* q, int64_t ldq, const void* k,
  * exist in the tensors, and rows that belong to no sequence are neither read
  * into a result nor written. Softmax statistics and sums are fp32, P is
  * rounded to dtype for the product with V. What a row does not see (later
- * rows, other sequences) cannot reach it, NaN and infinities included. A
- * sequence whose offsets are descending or outside [0, rows] is left out, with
+ * rows, other sequences) cannot reach it, NaN and infinities included. A value
+ * that is not finite and that a row does see leaves its column of that row not
+ * finite: infinite or NaN, which of the two is not promised where the key's
+ * weight is so small that P rounds it to 0. A sequence whose offsets are descending or outside [0, rows] is left out, with
  * all after it, and reported through the device status. scale <= 0 selects
  * 1/sqrt(head_dim). No workspace. kernel.attn.prefill with the row offsets of
  * an attn_meta value (src/ir/dialect/kernel/values.h:83-117). */
@@ -548,7 +550,8 @@ int kvm_sm100_attention_decode_paged(const void* q, int64_t ldq, const void* cac
  * positions outside a sequence's table or the table_len entries of block_table
  * are reported, and that sequence's result is undefined. Slots past a
  * sequence's last node and nodes a row does not see cannot reach it, NaN and
- * infinities included. */
+ * infinities included; values that are not finite and that it does see act as
+ * in kvm_sm100_attention_packed. */
 int64_t kvm_sm100_attention_tree_workspace(int S, int HQ, int HKV, int max_q_rows,
                                            int max_keys);
 int kvm_sm100_attention_tree_paged(const void* q, int64_t ldq, const void* cache,

@@ -44,7 +44,9 @@
 // cannot reach a row that does not see them. Values are different, as 0 * NaN
 // = NaN in the product: warp 12 zeroes what is not finite in V tiles that
 // some row sees only in part (and rows past the sequence's end), and the
-// epilogue adds those elements to the rows that do see them.
+// epilogue adds those elements to the rows that do see them. (An infinite value
+// whose weight rounds to 0 in P is NaN from a tile seen whole, as 0 * inf, and
+// infinity from one seen in part; neither is promised.)
 //
 // Measured (B200): 16383 tokens of 32 + 4 heads of 128 in 2.0-2.26 ms, 975 to
 // 1090 TFLOP/s of causal products, of 1641 that cuBLAS reaches in a burst and

@@ -164,6 +164,29 @@ def test_packed_broken_values_reach_only_who_sees_them(cuda, dtype, hd, group):
     assert bool(torch.isnan(o[250:400]).all()) and bool(torch.isnan(o[420]).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_packed_infinite_value_of_no_weight(cuda, dtype):
+    """An infinite value under a weight that P cannot hold, in a key tile that a
+    row sees whole and in one that it sees in part: the column is not finite in
+    the rows that see it, and nothing else changes."""
+    lens, hd = [400], 64
+    q, k, v, off = make(cuda, lens, 1, 1, hd, dtype, seed=12)
+    q[:, 0] = 40
+    k[:, 0] = 20                        # each score is 100, give or take a few,
+    for j in (20, 290):
+        k[j, 0] = -20                   # but these keys' is -100: weight e^-190
+    clean, mag = exact(q, k, v, lens, 1, 1, hd)
+    v[20, 3] = float("inf")
+    v[290, 5] = -float("inf")
+    out = ops.attention_packed(q, k, v, off, heads_q=1, heads_kv=1, head_dim=hd)
+    ops.device_status()
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[20:, 3] = bad[290:, 5] = True
+    assert bool((~torch.isfinite(out[bad])).all())
+    # scores are 100 instead of at most 64: P is off by twice as much
+    check(out[~bad], clean[~bad], 2 * mag[~bad], 400)
+
+
 def test_packed_bad_offsets_are_reported(cuda):
     q, k, v, _ = make(cuda, [64], 2, 1, 128, torch.bfloat16)
     out = torch.full_like(q, 3.0)
