@@ -588,7 +588,7 @@ int kvm_sm100_rope_bf16(void* x, int64_t ld, int rows, int L, int heads,
  *                      `high` turns (rounded down) to the one that makes `low`
  *                      (rounded up); m = 0.1 ln(factor) + 1
  *   KVM_ROPE_DIVISORS  f / divisors[i]
- * magnitude > 0 replaces m (otherwise 1). */
+ * magnitude > 0, a number that fp32 can hold, replaces m (otherwise 1). */
 enum kvm_rope_scaling {
   KVM_ROPE_NONE = 0, KVM_ROPE_LINEAR, KVM_ROPE_NTK, KVM_ROPE_BANDS, KVM_ROPE_YARN,
   KVM_ROPE_DIVISORS

@@ -251,8 +251,10 @@ extern "C" int kvm_sm100_rope_table(const kvm_rope_config* c, kvm_rope_table* t)
                 "rope_table: bands and yarn need original_len > 0 and 0 < low < high");
   if (kind == KVM_ROPE_NTK && d == 2)
     return fail(KVM_ERR_INVALID_ARG, "rope_table: ntk needs rotary_dim > 2");
-  if (!std::isfinite(c->magnitude) || c->magnitude < 0)
-    return fail(KVM_ERR_INVALID_ARG, "rope_table: magnitude must be finite and >= 0");
+  // (compared as it is held: a magnitude that fp32 makes infinite or zero is none)
+  if (!std::isfinite(static_cast<float>(c->magnitude)) || c->magnitude < 0 ||
+      (c->magnitude > 0 && static_cast<float>(c->magnitude) == 0.f))
+    return fail(KVM_ERR_INVALID_ARG, "rope_table: magnitude must be 0 or a positive fp32 number");
   if (kind == KVM_ROPE_DIVISORS) {
     if (!c->divisors) return fail(KVM_ERR_INVALID_ARG, "rope_table: divisors is NULL");
     for (int i = 0; i < d / 2; ++i)

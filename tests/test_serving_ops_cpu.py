@@ -76,6 +76,14 @@ def test_rope_table_refuses(d, kw):
     assert e.value.code == _lib.KVM_ERR_INVALID_ARG
 
 
+@pytest.mark.parametrize("magnitude", [1e39, 1e-50, float("inf"), float("nan")])
+def test_rope_table_refuses_a_magnitude_that_fp32_cannot_hold(magnitude):
+    """The table holds it in fp32, where these are infinity, zero or not numbers."""
+    with pytest.raises(KvmError) as e:
+        ops.rope_table(64, magnitude=magnitude)
+    assert e.value.code == _lib.KVM_ERR_INVALID_ARG
+
+
 def test_rope_table_python_refusals():
     with pytest.raises(ValueError):
         ops.rope_table(64, scaling="other")
