@@ -51,6 +51,12 @@ def tree_mask(parents, device=None) -> torch.Tensor:
     return t.view(len(rows), words).to(device)
 
 
+def _check_bounds(max_q_rows: int, max_keys: int) -> None:
+    """What the C calls would cut off to its low 32 bits is refused."""
+    if max_q_rows >> 31 not in (0, -1) or max_keys >> 31 not in (0, -1):
+        raise ValueError("max_q_rows and max_keys must fit 32 bits")
+
+
 class PagedKVCache:
     """A device pool of KV pages (bf16, zero-initialised)."""
 
@@ -129,6 +135,7 @@ class PagedKVCache:
     def tree_workspace(self, sequences: int, *, heads_q: int, max_q_rows: int,
                        max_keys: int) -> int:
         """Bytes of workspace `tree_decode` needs for these bounds."""
+        _check_bounds(max_q_rows, max_keys)
         return int(_lib.lib().kvm_sm100_attention_tree_workspace(
             sequences, heads_q, self.heads_kv, max_q_rows, max_keys))
 
@@ -153,6 +160,7 @@ class PagedKVCache:
         table = _list(block_table, "block_table", dev)
         if q.dim() != 2 or tree_mask.dim() != 2:
             raise ValueError("q and tree_mask must be 2-D")
+        _check_bounds(max_q_rows, max_keys)
         rows, words = q.shape[0], tree_mask.shape[1]
         ldq = _mat(q, "q", torch.bfloat16, rows, heads_q * 128, dev)
         if _mat(tree_mask, "tree_mask", torch.int32, rows, words, dev) != words:

@@ -54,6 +54,8 @@ def _mat(t: torch.Tensor, name: str, dtype: torch.dtype, rows: int, cols: int,
     the host: what passes is found out in few steps, what is wrong in others.)"""
     if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev >= 0 and \
             t.shape == (rows, cols):
+        if (rows | cols) >> 31:
+            raise ValueError(f"{name} has more rows or columns than 32 bits count")
         stride = t.stride()
         if stride[1] == 1 or cols <= 1:
             return stride[0] if rows > 1 else cols
@@ -70,7 +72,10 @@ def _list(t: torch.Tensor, name: str, dev: int, dtype: torch.dtype = torch.int32
     """Checks a contiguous list on CUDA device `dev`; returns its length."""
     if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev >= 0 and \
             t.dim() == 1 and t.is_contiguous():
-        return t.numel()
+        n = t.numel()
+        if n >> 31:
+            raise ValueError(f"{name} has more entries than 32 bits count")
+        return n
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype:
         raise TypeError(f"{name} must be a {dtype} tensor")
     if t.get_device() != dev or dev < 0:

@@ -4,6 +4,7 @@ import ctypes as C
 from decimal import Decimal, getcontext
 
 import pytest
+import torch
 
 from kvm_b200 import _lib, ops
 from kvm_b200._lib import KvmError
@@ -200,3 +201,48 @@ def test_attention_tree_refuses_without_a_gpu():
     assert ws(2, 8, 2, 5, 1024) == 0      # four short items are not cut
     assert ws(2, 8, 2, 5, 1025) == 9 * (2 * 256 * 130 * 4 + 32)    # 36 key tiles, four to a CTA
     assert ws(64, 64, 8, 16, 5000) == 148 * (2 * 256 * 130 * 4 + 32)
+
+
+class _OnGpu(torch.Tensor):
+    """A tensor without storage (meta) that says it is on GPU 0."""
+
+    def get_device(self):
+        return 0
+
+
+def _huge(*shape, dtype=torch.bfloat16):
+    return torch.empty(shape, dtype=dtype, device="meta").as_subclass(_OnGpu)
+
+
+def test_sizes_beyond_32_bits_are_refused(monkeypatch):
+    """The C calls take 32-bit counts and bounds: what does not fit is refused
+    instead of cut off to its low 32 bits (2^32 + 3 rows would run as 3)."""
+    from kvm_b200.kvcache import PagedKVCache
+    monkeypatch.setattr(ops, "_call_on", lambda *a: pytest.fail("the call went out"))
+    monkeypatch.setattr("kvm_b200.kvcache._call_on", lambda *a: pytest.fail("the call went out"))
+    n = 2 ** 32 + 3
+    pos = _huge(n, dtype=torch.int32)
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.rope(_huge(n, 4), pos, ops.rope_table(4), heads=1, head_dim=4, out=_huge(n, 4))
+    few = _huge(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.attention_packed(_huge(n, 64), _huge(n, 64), _huge(n, 64), few, heads_q=1, heads_kv=1,
+                             head_dim=64, out=_huge(n, 64))
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.attention_packed(_huge(5, 64), _huge(5, 64), _huge(5, 64), pos, heads_q=1, heads_kv=1,
+                             head_dim=64, out=_huge(5, 64))
+    cache = PagedKVCache(pages=4, layers=1, block_size=16, heads_kv=1, device="cpu")
+    cache.pool = _huge(4)
+    with pytest.raises(ValueError, match="32 bits"):
+        cache.copy_pages(pos, pos)
+    with pytest.raises(ValueError, match="32 bits"):
+        cache.compact(pos, few, few[:1], few, few)
+    one = _huge(1, dtype=torch.int32)
+    for bounds in (dict(max_keys=n, max_q_rows=3), dict(max_keys=9, max_q_rows=n),
+                   dict(max_keys=9 - 2 ** 32, max_q_rows=3)):
+        with pytest.raises(ValueError, match="32 bits"):
+            cache.tree_workspace(1, heads_q=1, **bounds)
+        for ws in (None, _huge(99, dtype=torch.uint8)):
+            with pytest.raises(ValueError, match="32 bits"):
+                cache.tree_decode(0, _huge(3, 128), few, one, _huge(3, 1, dtype=torch.int32), few,
+                                  few, heads_q=1, out=_huge(3, 128), workspace=ws, **bounds)
