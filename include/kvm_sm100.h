@@ -504,8 +504,9 @@ int kvm_sm100_kvcache_copy_pages(void* cache, const kvm_kv_layout* layout, int l
  * layout->layer on, K and V: the accepted path of a drafted tree becomes the
  * sequence's next tokens. In place. A sequence whose list is not strictly
  * increasing, or with a position outside its table, a table outside the
- * table_len entries of block_table or a page outside the pool, is left as it is and reported through the device status. The pages
- * moved to must not be shared between sequences of the call. No counterpart
+ * table_len entries of block_table (which may be NULL when that is 0) or a page
+ * outside the pool, is left as it is and reported through the device status. The
+ * pages moved to must not be shared between sequences of the call. No counterpart
  * in the reference (it has no tree decoding). */
 int kvm_sm100_kvcache_compact(void* cache, const kvm_kv_layout* layout, int layers,
                               const int32_t* kept, int n_kept, const int32_t* kept_offsets,
@@ -551,7 +552,7 @@ int kvm_sm100_attention_decode_paged(const void* q, int64_t ldq, const void* cac
  * are reported, and that sequence's result is undefined. Slots past a
  * sequence's last node and nodes a row does not see cannot reach it, NaN and
  * infinities included; values that are not finite and that it does see act as
- * in kvm_sm100_attention_packed. */
+ * in kvm_sm100_attention_packed. block_table may be NULL when table_len is 0. */
 int64_t kvm_sm100_attention_tree_workspace(int S, int HQ, int HKV, int max_q_rows,
                                            int max_keys);
 int kvm_sm100_attention_tree_paged(const void* q, int64_t ldq, const void* cache,

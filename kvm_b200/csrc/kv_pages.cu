@@ -212,7 +212,7 @@ extern "C" int kvm_sm100_kvcache_compact(void* cache, const kvm_kv_layout* L, in
   if (layers <= 0 || S < 0 || n_kept < 0 || table_len < 0 || !cache || !aligned16(cache))
     return fail(KVM_ERR_INVALID_ARG, "kvcache_compact: bad argument");
   if (S == 0 || n_kept == 0) return KVM_OK;
-  if (!kept || !kept_offsets || !q_positions || !block_table || !bt_offsets)
+  if (!kept || !kept_offsets || !q_positions || (!block_table && table_len > 0) || !bt_offsets)
     return fail(KVM_ERR_INVALID_ARG, "kvcache_compact: bad argument");
   const long long blocks = 2ll * layers * S;
   if (blocks >= (1ll << 31))

@@ -162,8 +162,8 @@ extern "C" int kvm_sm100_attention_tree_paged(
                 "attention_tree: max_q_rows 1..1024 and max_keys 1..2^30");
   if (mask_words <= 0 || int64_t(mask_words) * 32 < max_q_rows)
     return fail(KVM_ERR_INVALID_ARG, "attention_tree: the mask holds fewer than max_q_rows bits");
-  if (!q || !cache || !out || !q_offsets || !q_positions || !mask || !block_table ||
-      !bt_offsets || !aligned16(q) || !aligned16(cache) || !aligned16(out) ||
+  if (!q || !cache || !out || !q_offsets || !q_positions || !mask ||
+      (!block_table && table_len > 0) || !bt_offsets || !aligned16(q) || !aligned16(cache) || !aligned16(out) ||
       ldq < int64_t(HQ) * 128 || ldo < int64_t(HQ) * 128 || ldq % 8 || ldo % 8)
     return fail(KVM_ERR_INVALID_ARG, "attention_tree: bad pointer or row stride");
   const int64_t per = 2 * (128 / group);

@@ -174,6 +174,20 @@ def test_compact_refuses_tables_outside_the_list(cuda):
         assert torch.equal(_view(c), want)
 
 
+def test_compact_empty_block_table(cuda):
+    """No sequence has a page: one that keeps nothing is served, one that keeps
+    a token is reported."""
+    c = _cache(cuda, pages=4, layers=1, block_size=16, heads_kv=1)
+    want = _view(c).clone()
+    none, two = _i32([], cuda), _i32([0, 0], cuda)
+    c.compact(_i32([2], cuda), two, _i32([3], cuda), none, two)
+    ops.device_status()
+    c.compact(_i32([2], cuda), _i32([0, 1], cuda), _i32([3], cuda), none, two)
+    with pytest.raises(KvmError):
+        ops.device_status()
+    assert torch.equal(_view(c), want)
+
+
 def test_page_calls_in_a_graph(cuda):
     """Captured calls follow the lists and positions they find at replay."""
     c = _cache(cuda, pages=20, layers=2, block_size=16, heads_kv=2)

@@ -279,6 +279,23 @@ def test_tree_tables_outside_the_list_are_reported(cuda):
         check(out[4:], ref[4:], mag[4:], 304)
 
 
+def test_tree_empty_block_table(cuda):
+    """A padded step in which no sequence has a node or a page: nothing to do,
+    and nothing wrong. With nodes, their positions are outside their tables."""
+    c = Case(cuda, ctx=[100, 300], nodes=[4, 4], hq=4, hkv=1, bs=16, seed=34)
+    zero = _i32([0, 0, 0], cuda)
+    for off, bad in ((zero, False), (c.q_off, True)):
+        out = torch.full_like(c.q, 9.0)
+        c.cache.tree_decode(c.layer, c.q, off, c.q_pos, c.mask, c.bt[:0], zero, heads_q=4,
+                            max_q_rows=4, max_keys=304, out=out)
+        if bad:
+            with pytest.raises(KvmError):
+                ops.device_status()
+        else:
+            ops.device_status()
+            assert bool((out == 9).all())
+
+
 def test_tree_graph_and_two_streams(cuda):
     """A captured call follows contexts that change; two calls at once with a
     workspace each."""
