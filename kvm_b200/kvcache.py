@@ -158,6 +158,8 @@ class PagedKVCache:
             raise ValueError("q_offsets and bt_offsets must have one more entry than "
                              "q_positions")
         table = _list(block_table, "block_table", dev)
+        if not isinstance(q, torch.Tensor) or not isinstance(tree_mask, torch.Tensor):
+            raise TypeError("q and tree_mask must be tensors")
         if q.dim() != 2 or tree_mask.dim() != 2:
             raise ValueError("q and tree_mask must be 2-D")
         _check_bounds(max_q_rows, max_keys)
@@ -172,6 +174,8 @@ class PagedKVCache:
             need = self.tree_workspace(S, heads_q=heads_q, max_q_rows=max_q_rows,
                                        max_keys=max_keys)
             workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
+        elif not isinstance(workspace, torch.Tensor):
+            raise TypeError("workspace must be a tensor")
         elif workspace.get_device() != dev or not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous on the pool's device")
         _call_on(dev, "kvm_sm100_attention_tree_paged", q.data_ptr(), ldq,

@@ -391,7 +391,7 @@ def rope(q: torch.Tensor, positions: torch.Tensor, table: _lib.RopeTable, *, hea
             out_k = torch.empty((rows, heads_kv * head_dim), dtype=t, device=q.device)
         ldok = _mat(out_k, "out_k", t, rows, heads_kv * head_dim, dev)
         kp, okp = k.data_ptr(), out_k.data_ptr()
-    wide = positions.dtype is torch.int64
+    wide = getattr(positions, "dtype", None) is torch.int64
     if _list(positions, "positions", dev, torch.int64 if wide else torch.int32) != rows:
         raise ValueError("positions must have one entry per row")
     _call_on(dev, "kvm_sm100_rope", ctypes.byref(table), q.data_ptr(), ldq, out.data_ptr(), ldo,

@@ -246,3 +246,21 @@ def test_sizes_beyond_32_bits_are_refused(monkeypatch):
             with pytest.raises(ValueError, match="32 bits"):
                 cache.tree_decode(0, _huge(3, 128), few, one, _huge(3, 1, dtype=torch.int32), few,
                                   few, heads_q=1, out=_huge(3, 128), workspace=ws, **bounds)
+
+
+def test_what_is_no_tensor_is_refused():
+    from kvm_b200.kvcache import PagedKVCache
+    q = _huge(3, 128)
+    one, few = _huge(1, dtype=torch.int32), _huge(2, dtype=torch.int32)
+    cache = PagedKVCache(pages=4, layers=1, block_size=16, heads_kv=1, device="cpu")
+    cache.pool = _huge(4)
+    kw = dict(heads_q=1, max_q_rows=3, max_keys=9)
+    with pytest.raises(TypeError):
+        ops.rope(q, [0, 1, 2], ops.rope_table(4), heads=1, out=q)
+    with pytest.raises(TypeError):
+        cache.tree_decode(0, None, few, one, _huge(3, 1, dtype=torch.int32), few, few, **kw)
+    with pytest.raises(TypeError):
+        cache.tree_decode(0, q, few, one, [[1]], few, few, **kw)
+    with pytest.raises(TypeError):
+        cache.tree_decode(0, q, few, one, _huge(3, 1, dtype=torch.int32), few, few, out=q,
+                          workspace=4096, **kw)
