@@ -4,10 +4,12 @@
 // accepted tokens to consecutive slots. Both read kernel.kvcache's pool
 // (src/ir/dialect/kernel/dialect.cpp:69-70, src/ir/graph_config.h:20-39).
 //
-// Both only move bytes and are bound by HBM (96 pages of 2 MB in 62.6 us, 6.4
-// TB/s) or by launch latency (48 sequences of up to eight kept tokens, 24
-// layers: 10.5 us for 5.8 us of bytes); neither decides anything by the order
-// in which blocks run.
+// Both only move bytes. Copies are bound by HBM: 96 pages of 2 MB in 67-69 us
+// (5.9 TB/s) from 96 sources, in 63-64 us from 64 of them that repeat (5.3 TB/s
+// of what has to be read and written). Compaction is bound by the launch and by
+// reads that wait for one another, the lists, the tables and the rows (48
+// sequences of up to eight kept tokens, 24 layers: 10.4-10.8 us for 5.8 us of
+// bytes). Neither decides anything by the order in which blocks run.
 #include "kv_layout.h"
 #include "runtime.h"
 

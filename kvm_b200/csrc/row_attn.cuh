@@ -48,12 +48,14 @@
 // whose weight rounds to 0 in P is NaN from a tile seen whole, as 0 * inf, and
 // infinity from one seen in part; neither is promised.)
 //
-// Measured (B200): 16383 tokens of 32 + 4 heads of 128 in 2.0-2.26 ms, 975 to
+// Measured (B200): 16383 tokens of 32 + 4 heads of 128 in 2.0-2.27 ms, 970 to
 // 1090 TFLOP/s of causal products, of 1641 that cuBLAS reaches in a burst and
-// 1388 under the power cap; 32 trees of 16 nodes over 2000-4096 keys in 86-95
-// us with the joins, 4.2-4.7 TB/s of K and V. What bounds it is the chain of a stream's scores,
-// softmax and products (1950 cycles of softmax and as many of waiting a tile),
-// for trees the K/V tiles in flight. The code is kept short (waits counted in
+// 1388 under the power cap; 32 trees of 16 nodes over 2000-4096 keys in 86-98
+// us with the joins, 4.1-4.7 TB/s of K and V. What bounds it is the chain of a
+// stream's scores, softmax and products (1950 cycles of softmax and as many of
+// waiting a tile), for trees the stream of K/V tiles (what holds it below the
+// copy rate is not known; a third V stage helped, a second Q tile's place is
+// all that is left for another). The code is kept short (waits counted in
 // polls, loops rolled): at 106 KB a sixth of its instruction requests missed.
 //
 // Every wait is bounded; a timeout sets the device status and the kernel
